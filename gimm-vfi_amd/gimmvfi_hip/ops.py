@@ -12,6 +12,7 @@ import math
 import torch
 
 from . import lib as L
+from . import rows
 
 
 def roundup(x, m):
@@ -609,18 +610,33 @@ class Runtime:
                                           self.dtype, self.stream()), "instnorm_apply")
         return out
 
+    def _here(self, t):
+        return t.device.type == self.device.type and self.device.index in (None, t.device.index)
+
+    def _fits(self, name, what, v, c, dtype):
+        """v: View whose launch reads or writes the channels [coff, coff + c) of every pixel of a dense tensor of type dtype."""
+        if v.t.dtype != dtype or not v.t.is_contiguous() or v.coff < 0 or v.coff + c > v.ld or not self._here(v.t):
+            raise ValueError(f"{name}: {what} must be contiguous {dtype} on {self.device} with channels [{v.coff}, {v.coff + c}), "
+                             f"got {v.t.dtype} {tuple(v.t.shape)} on {v.t.device}")
+
     def group_norm(self, x, c, groups, gb=None, act=L.ACT_NONE, eps=1e-5, out=None):
         """act(group norm) of the channel slice x (gb = (gamma, beta) float tensors or None); gimmvfi_hip.group_norm is the form for
         plain tensors, with the backward pass."""
         x = V(x)
+        if x.t.dim() != 4:
+            raise ValueError(f"group_norm: x must be (N, H, W, C), got shape {tuple(x.t.shape)}")
         n, h, w = x.t.shape[:3]
         out = V(self.act(n, h, w, c) if out is None else out)
+        self._fits("group_norm", "x", x, c, self.tdtype)
+        self._fits("group_norm", "out", out, c, self.tdtype)
+        if out.t.shape[:3] != x.t.shape[:3]:
+            raise ValueError(f"group_norm: out must have the pixels of x, {tuple(x.t.shape[:3])}, got {tuple(out.t.shape[:3])}")
+        gamma, beta = (None, None) if gb is None else (rows.check_vector(t, c, x.t, s) for t, s in zip(gb, ("gamma", "beta")))
         nws = self.lib.group_norm_workspace(c, groups, n, h * w)
         if nws < 0:
             raise ValueError(f"group_norm: {c} channels, {groups} groups, {n} images of {h} x {w}")
         ws, stats = self.f32(max(nws, 1)), self.f32(n, groups, 2)
-        self._chk(self.lib.group_norm(x.ptr, x.ld, c, groups, n, h * w, None if gb is None else gb[0].data_ptr(),
-                                      None if gb is None else gb[1].data_ptr(), float(eps), act, out.ptr, out.ld, stats.data_ptr(),
+        self._chk(self.lib.group_norm(x.ptr, x.ld, c, groups, n, h * w, gamma, beta, float(eps), act, out.ptr, out.ld, stats.data_ptr(),
                                       ws.data_ptr(), self.dtype, self.stream()), "group_norm")
         return out
 
@@ -885,14 +901,21 @@ class Runtime:
         """softmax_rows with a learned relative position bias: x float [b * heads * Q, M] -> out (pad columns cleared); plan:
         gimmvfi_hip.rel_softmax.RelativeBuckets (that module is the form for plain tensors, with the backward pass)."""
         o = V(out)
-        m = plan.kh * plan.kw
-        if x.dtype != torch.float32 or not x.is_contiguous() or x.shape[-1] != m or x.numel() != b * heads * plan.qh * plan.qw * m:
-            raise ValueError(f"softmax_rel_bias: x must be contiguous float32 of {b} x {heads} x {plan.qh * plan.qw} rows of {m}, got {x.dtype} {tuple(x.shape)}")
-        if key_mask is not None and (tuple(key_mask.shape) != (b, m) or key_mask.dtype not in (torch.bool, torch.uint8) or not key_mask.is_contiguous()):
-            raise ValueError(f"softmax_rel_bias: key_mask must be contiguous bool ({b}, {m}), got {key_mask.dtype} {tuple(key_mask.shape)}")
+        m, n = plan.kh * plan.kw, b * heads * plan.qh * plan.qw
+        if x.dtype != torch.float32 or not x.is_contiguous() or x.shape[-1] != m or x.numel() != n * m or not self._here(x):
+            raise ValueError(f"softmax_rel_bias: x must be contiguous float32 of {b} x {heads} x {plan.qh * plan.qw} rows of {m} on {self.device}, got {x.dtype} {tuple(x.shape)} on {x.device}")
+        self._fits("softmax_rel_bias", "out", o, o.c, self.tdtype)
+        if o.c < m or o.npix < n:
+            raise ValueError(f"softmax_rel_bias: out must hold {n} rows of {m} columns, got {tuple(o.t.shape)}")
+        if key_mask is not None and (tuple(key_mask.shape) != (b, m) or key_mask.dtype not in (torch.bool, torch.uint8) or not key_mask.is_contiguous() or key_mask.device != x.device):
+            raise ValueError(f"softmax_rel_bias: key_mask must be contiguous bool ({b}, {m}) on {x.device}, got {key_mask.dtype} {tuple(key_mask.shape)} on {key_mask.device}")
+        if table.dtype != torch.float32 or tuple(table.shape) != (plan.num_buckets, heads) or not table.is_contiguous() or table.device != x.device:
+            raise ValueError(f"softmax_rel_bias: table must be contiguous float32 ({plan.num_buckets}, {heads}) on {x.device}, got {table.dtype} {tuple(table.shape)} on {table.device}")
+        if plan.bucket_of.device != x.device:
+            raise ValueError(f"softmax_rel_bias: the plan is on {plan.bucket_of.device}, x on {x.device}: use plan.to(x.device)")
         nws = self.lib.softmax_rel_bias_workspace(b, heads, plan.qh, plan.qw, plan.kh, plan.kw, 0)
-        if nws < 0 or tuple(table.shape) != (plan.num_buckets, heads):
-            raise ValueError(f"softmax_rel_bias: table {tuple(table.shape)}, {plan.num_buckets} buckets, {heads} heads")
+        if nws < 0:
+            raise ValueError(f"softmax_rel_bias: {b} x {heads} x {plan.qh * plan.qw} rows of {m} are out of range")
         ws = self.f32(max(nws, 1))
         self._chk(self.lib.softmax_rel_bias(x.data_ptr(), L.F32, x.shape[-1], table.data_ptr(), plan.bucket_of.data_ptr(),
                                             plan.num_buckets, None if key_mask is None else key_mask.data_ptr(), float(scale), o.ptr,
