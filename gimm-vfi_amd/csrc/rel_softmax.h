@@ -652,7 +652,7 @@ template <typename TX, typename TY, int T, int NC, int NQ> __global__ __launch_b
                 float p[NQ][NC][4], d[NQ][NC][4], dot[NQ], top[NQ], inv[NQ];
 #pragma unroll
                 for (int q = 0; q < NQ; ++q) {
-                    const long long rq = r + (q < nq ? q : 0);               // (a query that is not there: the first again, times 0)
+                    const long long rq = r + (q < nq ? q : 0);               // (a query that is not there: the first again)
                     const TX* x = (const TX*)a.x + rq * a.ldx;
                     const TY* dy = (const TY*)a.dy + rq * a.lddy;
                     top[q] = a.stats[2 * rq];
@@ -716,11 +716,18 @@ template <typename TX, typename TY, int T, int NC, int NQ> __global__ __launch_b
 #pragma unroll
                     for (int q = 0; q < NQ; ++q) {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            p[q][i][e] *= d[q][i][e] - dot[q];
-                            w[NQ - 1 - q + e] += p[q][i][e];
-                            p[q][i][e] *= a.scale;
+                        for (int e = 0; e < 4; ++e) p[q][i][e] *= d[q][i][e] - dot[q];
+                        if (nq == NQ && RS_FULL(i)) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) w[NQ - 1 - q + e] += p[q][i][e];
+                        } else {
+                            // (selected: beside a NaN a column or a query that is not there has a NaN too, and its slot is another's)
+                            const int nv = RsChunk::rare(a, (t + i * T) * 4).nv;
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) w[NQ - 1 - q + e] += q < nq && e < nv ? p[q][i][e] : 0.f;
                         }
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) p[q][i][e] *= a.scale;
                         TX* dx = (TX*)a.y + (r + q) * a.ldy;
                         if (q >= nq) continue;
                         if (RS_FULL(i)) store4<TX>(dx + (t + i * T) * 4, p[q][i]);

@@ -6,6 +6,7 @@ import torch
 
 import train_ops_oracle as orc
 from gimmvfi_hip import lib as L
+from gimmvfi_hip import rel_softmax as rs
 from test_trainable_ops import BF16, F16, F32, _gen, _rs_plan, _runtime, _within, dev  # noqa: F401
 
 
@@ -38,3 +39,29 @@ def test_runtime_forms_refuse_what_they_would_read_or_write_wrongly():
                dict(out=torch.zeros(48, 32, dtype=F16)[:, ::2]), dict(m=torch.ones(2, 12))):
         with pytest.raises(ValueError):
             rs(**kw)
+
+
+# ------------------------------------------------------------------------------------------------ NaN rows stay alone
+# keys of a 1 x M row; above 128 columns fours of columns are taken together, four queries at a time up to 1024 and from 2049 to 4096
+# columns, two at a time elsewhere
+@pytest.mark.parametrize("whole", [False, True], ids=["one", "whole"])
+@pytest.mark.parametrize("m", [145, 146, 147, 257, 1025, 1026, 1027, 2051, 4097])
+def test_softmax_rel_bias_nan_row_reaches_its_own_offsets_only(dev, m, whole):
+    plan = _rs_plan("grid", (1, 6), (1, m), dev)
+    table = torch.randn(plan.num_buckets, 1, generator=_gen(1))
+    x, dy = torch.randn(1, 1, 6, m, generator=_gen(2)), torch.randn(1, 1, 6, m, generator=_gen(3))
+    x[0, 0, 4, slice(None) if whole else 7] = float("nan")
+    y, stats = rs.forward(x.to(dev), table.to(dev), plan)
+    dx, dt = rs.backward(dy.to(dev), x.to(dev), stats, table.to(dev), plan)
+    for t in (y.cpu(), dx.cpu()):
+        assert bool(t[0, 0, 4].isnan().all()) and not bool(t[0, 0, [0, 1, 2, 3, 5]].isnan().any())
+    # query 4 of six meets the slots 1 .. m of m + 5: key j has slot j - 4 + 5
+    bad = dt.cpu().isnan()[:, 0]
+    assert bad[1:m + 1].all() and not bad[0] and not bad[m + 1:].any(), bad.nonzero().flatten().tolist()[-3:]
+    # the offsets that no NaN meets have the gradient of the rows that hold none
+    clean = x.clone()
+    clean[0, 0, 4] = -float("inf")
+    ref = orc.softmax_rel_bias(clean, table, plan.bucket_of, (1, 6), (1, m), 1.0, None, F32, dy)
+    keep = torch.ones(m + 5, dtype=torch.bool)
+    keep[1:m + 1] = False
+    _within(dt.cpu()[keep], ref["dtable"][keep], ref["dtable_tol"][keep], "dtable")
