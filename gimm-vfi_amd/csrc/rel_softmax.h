@@ -24,7 +24,7 @@
 //
 // Gradient of the table: a workgroup takes the rows of a tile of RX x RY neighbouring queries (of several samples) of one head and
 // adds every ds into its slot of a slab in LDS.  In one row every column has a slot of its own, so the adds need no atomics, only
-// an order between rows (the barrier of the row's sum; a slab per 16-lane unit).  Slabs are written out, summed by slot and then
+// an order between rows (the barrier of the row's sum; wave_order() and a slab per unit where one wave has whole rows).  Slabs are written out, summed by slot and then
 // by bucket in a fixed order, in double: a bucket may collect millions of terms.
 //
 // Measured on one MI355X (copy of 1 GiB: 5.2 TB/s), float scores, bfloat16 probabilities: 28672 rows of 1792 (32 x 56 map) 59 us =
@@ -581,17 +581,20 @@ __global__ __launch_bounds__(T < 64 ? RS_BLOCK : T) void rs_backward_kernel(RsAr
         }
 #pragma unroll
         for (int q = 0; q < ROWS; ++q) {
-            if (k + q >= k1) continue;
-            TX* dx = (TX*)a.y + row[q] * a.ldy;
+            if (k + q < k1) {
+                TX* dx = (TX*)a.y + row[q] * a.ldy;
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int j = c0 + t + i * T;
-                if (j < a.M) {
-                    const float ds = p[q][i] * (d[q][i] - dot[q]);
-                    dx[j] = to_elem<TX>(ds * a.scale);
-                    if (adds) slab[so[i] + sb[q]] += ds;
+                for (int i = 0; i < NV; ++i) {
+                    const int j = c0 + t + i * T;
+                    if (j < a.M) {
+                        const float ds = p[q][i] * (d[q][i] - dot[q]);
+                        dx[j] = to_elem<TX>(ds * a.scale);
+                        if (adds) slab[so[i] + sb[q]] += ds;
+                    }
                 }
             }
+            // (of two rows, different lanes add to one word; several waves have the barrier of the row's sum in between)
+            if (WAVES == 1 && !SPLIT) wave_order();
         }
     }
     if (adds) {

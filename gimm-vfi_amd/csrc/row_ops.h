@@ -122,6 +122,17 @@ __device__ __forceinline__ float wave_max(float v) {
 }
 #endif
 
+// A wave's accesses to memory before this place happen before those after it, whichever of its lanes make them.  No instruction: a wave's LDS
+// operations are carried out in order, what this stops is the compiler moving them.
+__device__ __forceinline__ void wave_order() {
+#ifndef GVFI_HOSTSIM
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#else
+    emu::wave_sync();
+#endif
+}
+
 // 2^x of the hardware: about one step of float; 0 below 2^-126; 2^-inf = 0, a NaN stays one
 __device__ __forceinline__ float exp2_hw(float x) {
 #ifndef GVFI_HOSTSIM
