@@ -13,7 +13,18 @@
 
 #include <stdint.h>
 #include <string.h>
+#include <atomic>
+#include <mutex>
 #include "../../include/gimmvfi_hip.h"
+
+// Raises a limit to `want` by set(want) and never lowers it, whichever threads ask at once.
+template <typename F> static inline void gvfi_raise_limit(std::atomic<int>& have, std::mutex& turn, int want, F set) {
+    if (have.load() >= want) return;
+    std::lock_guard<std::mutex> mine(turn);
+    if (have.load() >= want) return;
+    set(want);
+    have = want;
+}
 
 #ifndef GVFI_HOSTSIM
 // (emulator only: a launch whose workgroups meet in float atomics keeps its block order; nothing on the device)
@@ -29,14 +40,13 @@
 #define GVFI_DYN_SMEM(name) extern __shared__ __attribute__((aligned(16))) unsigned char name[]
 #define GVFI_LAUNCH_COOP_SHM(kernel, grid, block, shm, stream, ...)                                         \
     do {                                                                                                    \
-        static int gvfi_attr_set_[16] = {0}; /* per device: the attribute belongs to the device's code object */ \
+        static std::atomic<int> gvfi_attr_set_[16]; /* per device: the attribute belongs to the device's code object */ \
+        static std::mutex gvfi_attr_turn_;      /* launches of sizes that differ, from several threads (autograd's among them) */ \
         int gvfi_dev_ = 0;                                                                                  \
         (void)hipGetDevice(&gvfi_dev_);                                                                     \
-        gvfi_dev_ &= 15;                                                                                    \
-        if (gvfi_attr_set_[gvfi_dev_] < (int)(shm)) {                                                       \
-            hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)(shm)); \
-            gvfi_attr_set_[gvfi_dev_] = (int)(shm);                                                         \
-        }                                                                                                   \
+        gvfi_raise_limit(gvfi_attr_set_[gvfi_dev_ & 15], gvfi_attr_turn_, (int)(shm), [&](int gvfi_n_) {    \
+            (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, gvfi_n_); \
+        });                                                                                                 \
         hipLaunchKernelGGL(kernel, grid, block, shm, stream, __VA_ARGS__);                                  \
     } while (0)
 #endif

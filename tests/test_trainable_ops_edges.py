@@ -65,3 +65,10 @@ def test_softmax_rel_bias_nan_row_reaches_its_own_offsets_only(dev, m, whole):
     keep = torch.ones(m + 5, dtype=torch.bool)
     keep[1:m + 1] = False
     _within(dt.cpu()[keep], ref["dtable"][keep], ref["dtable_tol"][keep], "dtable")
+
+
+# ------------------------------------------------------------------------------------------------ launches from several threads
+@pytest.mark.parametrize("small_first", [0, 1])
+def test_two_threads_leave_the_larger_limit_of_dynamic_lds(simlib, small_first):
+    """Autograd's threads launch the backward pass with slabs of different sizes: the kernel's limit must not fall again."""
+    assert simlib.dll.gvfi_emu_limit_selftest(small_first) == 1000
