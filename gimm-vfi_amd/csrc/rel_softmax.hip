@@ -49,17 +49,28 @@ __device__ __forceinline__ double rs_slot_sum(const RsArgs& a, int h, int s, int
     return acc;
 }
 
+// Workgroups of the sums behind the slabs: a launch has fewer than 2^32 lanes, the workgroups loop over what is left
+#ifndef GVFI_HOSTSIM
+#define RS_MOST_GROUPS (1LL << 23)
+#else
+#define RS_MOST_GROUPS 7LL      // (the emulator's tests take the loops)
+#endif
+static unsigned rs_groups(long long n) { return (unsigned)(n < RS_MOST_GROUPS ? n : RS_MOST_GROUPS); }
+
 // 16 slots x 16 of the parts of the slabs; gridDim.z workgroups share the slabs of 16 slots and leave a sum each
 __global__ __launch_bounds__(RS_BLOCK) void rs_slots_kernel(RsArgs a) {
     __shared__ double red[16][16];
     const int l = threadIdx.x & 15, w = threadIdx.x >> 4, h = blockIdx.y;
-    const int s = blockIdx.x * 16 + l;
-    red[w][l] = s < a.slots ? rs_slot_sum(a, h, s, (int)blockIdx.z * 16 + w, 16 * a.zparts) : 0.0;
-    __syncthreads();
-    if (w == 0 && s < a.slots) {
-        double acc = 0.0;
-        for (int k = 0; k < 16; ++k) acc += red[k][l];
-        a.dslot[((long long)blockIdx.z * a.heads + h) * a.slots + s] = acc;
+    for (int s0 = (int)blockIdx.x * 16; s0 < a.slots; s0 += (int)gridDim.x * 16) {        // (slots < 2^30, the step at most 2^27)
+        const int s = s0 + l;
+        red[w][l] = s < a.slots ? rs_slot_sum(a, h, s, (int)blockIdx.z * 16 + w, 16 * a.zparts) : 0.0;
+        __syncthreads();
+        if (w == 0 && s < a.slots) {
+            double acc = 0.0;
+            for (int k = 0; k < 16; ++k) acc += red[k][l];
+            a.dslot[((long long)blockIdx.z * a.heads + h) * a.slots + s] = acc;
+        }
+        __syncthreads();
     }
 }
 
@@ -67,23 +78,28 @@ __global__ __launch_bounds__(RS_BLOCK) void rs_slots_kernel(RsArgs a) {
 template <int P> __global__ __launch_bounds__(RS_BLOCK) void rs_buckets_kernel(RsArgs a, int parts, double* share) {
     __shared__ double red[RS_BLOCK];
     const int t = threadIdx.x % P, h = blockIdx.y;
-    const long long unit = (long long)blockIdx.x * (RS_BLOCK / P) + threadIdx.x / P;
-    const int k = (int)(unit / parts), part = (int)(unit - (long long)k * parts);
-    double s = 0.0;
-    if (k < a.buckets)
-        for (int i = a.starts[k] + part * P + t; i < a.starts[k + 1]; i += P * parts) {
-            const int slot = a.order[i];
-            if ((unsigned)slot < (unsigned)a.slots)
-                for (int z = 0; z < a.zparts; ++z) s += a.dslot[((long long)z * a.heads + h) * a.slots + slot];
+    const long long units = (long long)a.buckets * parts;
+    for (long long u0 = (long long)blockIdx.x * (RS_BLOCK / P); u0 < units; u0 += (long long)gridDim.x * (RS_BLOCK / P)) {
+        const long long unit = u0 + threadIdx.x / P;
+        const long long k = unit / parts;
+        const int part = (int)(unit - k * parts);
+        double s = 0.0;
+        if (k < a.buckets)
+            for (int i = a.starts[k] + part * P + t; i < a.starts[k + 1]; i += P * parts) {
+                const int slot = a.order[i];
+                if ((unsigned)slot < (unsigned)a.slots)
+                    for (int z = 0; z < a.zparts; ++z) s += a.dslot[((long long)z * a.heads + h) * a.slots + slot];
+            }
+        red[threadIdx.x] = s;
+        for (int o = P / 2; o > 0; o >>= 1) {
+            __syncthreads();
+            if (t < o) red[threadIdx.x] += red[threadIdx.x + o];
         }
-    red[threadIdx.x] = s;
-    for (int o = P / 2; o > 0; o >>= 1) {
+        if (t == 0 && k < a.buckets) {
+            if (parts == 1) a.dtable[k * a.heads + h] = (float)red[threadIdx.x];
+            else share[(k * a.heads + h) * parts + part] = red[threadIdx.x];
+        }
         __syncthreads();
-        if (t < o) red[threadIdx.x] += red[threadIdx.x + o];
-    }
-    if (t == 0 && k < a.buckets) {
-        if (parts == 1) a.dtable[(long long)k * a.heads + h] = (float)red[threadIdx.x];
-        else share[((long long)k * a.heads + h) * parts + part] = red[threadIdx.x];
     }
 }
 __global__ __launch_bounds__(RS_BLOCK) void rs_shares_kernel(RsArgs a, int parts, const double* share) {
@@ -130,8 +146,9 @@ static int rs_check(RsArgs& a, long long B, int heads, int qh, int qw, int kh, i
     a.by_kw = rs_divisor((unsigned)kw); a.by_Q = rs_divisor((unsigned)Q); a.by_heads = rs_divisor((unsigned)heads);
     a.by_qw = rs_divisor((unsigned)qw); a.by_qh = rs_divisor((unsigned)qh);
     a.tiles = M <= RS_LONGEST ? 1 : (int)((M + RS_TILE - 1) / RS_TILE);
-    // (a launch has fewer than 2^32 lanes: 2^23 workgroups of 512 for rows in tiles)
-    return a.rows * a.tiles < (a.tiles > 1 ? 1LL << 23 : 1LL << 31) ? 0 : -2;
+    // A launch has fewer than 2^32 lanes: workgroups of 512 for rows in tiles, else T lanes (RS_BY_LENGTH) for 16 rows
+    const long long T = a.tiles > 1 ? 512 * 16 : M <= 128 ? 16 : M <= 512 ? 64 : M <= 2048 ? 256 : M <= 8192 ? 512 : 1024;
+    return a.rows < (1LL << 31) && a.rows * a.tiles * T < (1LL << 36) ? 0 : -2;
 }
 // Tile of queries and samples of a workgroup of the backward pass.  More rows per slab spread the cost of clearing, writing and
 // reading it again (about 12 bytes per slot against 10 per element of every row); more workgroups fill the chip.
@@ -172,8 +189,12 @@ static void rs_backward_plan(RsArgs& a) {
 }
 // the expanded table with its margins, in whole 16 bytes
 static long long rs_bias_floats(const RsArgs& a) { return ((long long)a.heads * a.slots + 2 * RS_MARGIN + 3) / 4 * 4; }
-// workgroups of the backward pass (a launch has fewer than 2^32 lanes)
 static long long rs_workgroups(const RsArgs& a) { return (long long)a.heads * a.tb * a.ty * a.tx * a.tiles; }
+// whether the backward pass is a launch of fewer than 2^32 lanes (workgroups of at most 256 lanes up to 1024 columns, of 512 up to 8192 and
+// in tiles, else of 1024)
+static bool rs_backward_fits(const RsArgs& a) {
+    return rs_workgroups(a) * (a.M <= 1024 ? 256 : a.M <= 8192 || a.tiles > 1 ? 512 : 1024) < (1LL << 32);
+}
 static long long rs_slab_floats(const RsArgs& a) { return rs_workgroups(a) * a.slab_n; }
 extern "C" long long gvfi_softmax_rel_bias_workspace(long long B, int heads, int qh, int qw, int kh, int kw, int backward) {
     RsArgs a = {};
@@ -181,7 +202,7 @@ extern "C" long long gvfi_softmax_rel_bias_workspace(long long B, int heads, int
     const long long nb = rs_bias_floats(a), np = a.tiles > 1 ? a.rows * a.tiles * 2 : 0;
     if (!backward || B == 0) return nb + np;
     rs_backward_plan(a);
-    if (rs_workgroups(a) >= (1LL << 24)) return -2;
+    if (!rs_backward_fits(a)) return -2;
     return nb + 2LL * a.zparts * heads * a.slots + 1 + np + rs_slab_floats(a) + (a.slots < 8192 ? 0 : RS_SHARES * 2LL * heads);
 }
 #define RS_DISPATCH(...)                                                                              \
@@ -217,7 +238,7 @@ extern "C" int gvfi_softmax_rel_bias_backward(const void* dy, long long lddy, co
     if (!x || !dy || !dx || !table || !bucket_of || !stats || !workspace || ldx < a.M || lddy < a.M || lddx < a.M) return -2;
     if (dtable && (!order || !starts)) return -2;
     rs_backward_plan(a);
-    if (rs_workgroups(a) >= (1LL << 24)) return -2;
+    if (!rs_backward_fits(a)) return -2;
     a.x = x; a.ldx = ldx; a.dy = dy; a.lddy = lddy; a.y = dx; a.ldy = lddx; a.zero_to = a.M; a.table = table;
     a.bucket_of = bucket_of; a.mask = key_mask; a.stats = (float*)stats; a.scale = scale; a.dtable = dtable;
     a.order = order; a.starts = starts;
@@ -231,16 +252,16 @@ extern "C" int gvfi_softmax_rel_bias_backward(const void* dy, long long lddy, co
     if (dtable && a.slots <= RS_FEW_SLOTS && a.slots / buckets < 8 && buckets <= 4096 && (long long)a.ty * a.tb >= 64) {
         GVFI_LAUNCH_COOP(rs_direct_kernel, dim3((unsigned)buckets, (unsigned)heads), dim3(RS_BLOCK), st, a);
     } else if (dtable) {
-        GVFI_LAUNCH_COOP(rs_slots_kernel, dim3((unsigned)((a.slots + 15) / 16), (unsigned)heads, (unsigned)a.zparts), dim3(RS_BLOCK), st, a);
+        GVFI_LAUNCH_COOP(rs_slots_kernel, dim3(rs_groups((a.slots + 15LL) / 16), (unsigned)heads, (unsigned)a.zparts), dim3(RS_BLOCK), st, a);
         if (buckets <= 1024) {
             const int parts = rs_parts(a, buckets);
-            GVFI_LAUNCH_COOP((rs_buckets_kernel<RS_BLOCK>), dim3((unsigned)(buckets * parts), (unsigned)heads), dim3(RS_BLOCK), st, a, parts,
+            GVFI_LAUNCH_COOP((rs_buckets_kernel<RS_BLOCK>), dim3(rs_groups((long long)buckets * parts), (unsigned)heads), dim3(RS_BLOCK), st, a, parts,
                              share);
             if (parts > 1)
                 GVFI_LAUNCH_SIMPLE(rs_shares_kernel, dim3((unsigned)(((long long)buckets * heads + RS_BLOCK - 1) / RS_BLOCK)), dim3(RS_BLOCK), st,
                                    a, parts, (const double*)share);
         } else {
-            GVFI_LAUNCH_COOP((rs_buckets_kernel<16>), dim3((unsigned)((buckets + 15) / 16), (unsigned)heads), dim3(RS_BLOCK), st, a, 1, share);
+            GVFI_LAUNCH_COOP((rs_buckets_kernel<16>), dim3(rs_groups((buckets + 15LL) / 16), (unsigned)heads), dim3(RS_BLOCK), st, a, 1, share);
         }
     }
     return (int)hipGetLastError();

@@ -7,7 +7,7 @@ import torch
 import train_ops_oracle as orc
 from gimmvfi_hip import lib as L
 from gimmvfi_hip import rel_softmax as rs
-from test_trainable_ops import BF16, F16, F32, _gen, _rs_plan, _runtime, _within, dev  # noqa: F401
+from test_trainable_ops import BF16, F16, F32, _gen, _rs_case, _rs_plan, _runtime, _within, dev  # noqa: F401
 
 
 # ------------------------------------------------------------------------------------------------ the launch list's arguments
@@ -72,3 +72,43 @@ def test_softmax_rel_bias_nan_row_reaches_its_own_offsets_only(dev, m, whole):
 def test_two_threads_leave_the_larger_limit_of_dynamic_lds(simlib, small_first):
     """Autograd's threads launch the backward pass with slabs of different sizes: the kernel's limit must not fall again."""
     assert simlib.dll.gvfi_emu_limit_selftest(small_first) == 1000
+
+
+# ------------------------------------------------------------------------------------------------ launches of 2^32 lanes and more
+def test_sizes_whose_sums_would_be_launches_of_too_many_lanes_are_taken(simlib):
+    """Sixteen slots or buckets per 256 lanes: from 2^28 on the sums behind the slabs loop instead of asking for 2^32 lanes.  (In the
+    emulator seven workgroups loop over everything, so every case of the suite goes through them.)"""
+    assert simlib.softmax_rel_bias_workspace(1, 1, 1, 1, 1, (1 << 28) + 64, 1) > 0
+    # rows of 9000 columns: 1024 lanes take sixteen rows, so 2^26 rows would be 2^32 lanes
+    assert simlib.softmax_rel_bias_workspace(1 << 12, 1 << 11, 1, 8, 1, 9000, 0) == -2
+    assert simlib.softmax_rel_bias_workspace(1 << 11, 1 << 11, 1, 8, 1, 9000, 0) > 0
+
+
+@pytest.mark.parametrize("case", [((1, 40), (1, 300), "grid"), ((3, 5), (7, 20), "shared"), ((1, 3), (1, 5000), "log"), ((2, 2), (30, 41), "grid")],
+                         ids=lambda c: f"{c[0]}-{c[1]}-{c[2]}")
+def test_softmax_rel_bias_sums_in_loops(dev, case):
+    q, k, kind = case
+    _rs_case(dev, 2, 2, q, k, kind, F32, F32, False, None, 0)
+
+
+@pytest.mark.gpu
+def test_gpu_softmax_rel_bias_one_query_2_28_keys():
+    """A bucket of its own for every one of 2^28 + 64 keys: the table's gradient is the gradient of the scores, both in float."""
+    d = torch.device("cuda", 0)
+    m = (1 << 28) + 64
+    plan = rs.RelativeBuckets.per_offset((1, 1), (1, m), device=d)
+    x, dy, table = (torch.randn(1, 1, 1, m, device=d, generator=torch.Generator(device=d).manual_seed(k)) for k in (1, 2, 3))
+    table = table.view(m, 1)
+    y, stats = rs.forward(x, table, plan)
+    dx, dt = rs.backward(dy, x, stats, table, plan)
+    assert torch.equal(dx.view(-1), dt.view(-1))
+    v = x.view(-1).double() + table.view(-1)
+    p = torch.exp(v - v.max())
+    p /= p.sum()
+    # |v| and the largest value stay below 10: four roundings of each, and at most 88 of the exponential, the sums and the inverse
+    rel = orc.U * (4 * 10 + 4 * 10 + 88)
+    assert bool(((y.view(-1).double() - p).abs() <= p * (rel + 2 * orc.U) + 2.0 ** -126).all())
+    g = dy.view(-1).double()
+    dot = (p * g).sum()
+    tol = p * (rel * (g - dot).abs() + (p * g.abs()).sum() * (rel + 96 * orc.U) + 8 * orc.U * (g.abs() + dot.abs())) + 2.0 ** -126
+    assert bool(((dx.view(-1).double() - p * (g - dot)).abs() <= tol + 2 * orc.U * (p * (g - dot)).abs()).all())
