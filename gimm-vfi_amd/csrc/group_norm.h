@@ -5,11 +5,12 @@
 //   dx = rstd * (gamma dz - A - xhat B),  A = mean over the group of gamma dz,  B = mean over the group of gamma dz xhat
 //
 // The work is a few operations per element: bytes bind.  A workgroup covers a run of pixels of one image and up to 64 octets of
-// channels; a lane keeps its octet, so everything that depends on the channel stays in registers.  Statistics: every lane sums
-// x - k and (x - k)^2 with k its own first value -- k is one of the values, so (k - mean)^2 <= M2 and the difference
-// sum (x-k)^2 - (sum (x-k))^2 / n loses at most a factor n + 1 of the lane's few dozen values, whatever the mean.  Means and
-// centred sums (M2 = sum (x - mean)^2) are then joined as  mean = sum n_i mean_i / n,  M2 = sum M2_i + n_i (mean_i - mean)^2,
-// always in the same order: two runs give the same bits.
+// channels; a lane keeps its octet, so everything that depends on the channel stays in registers.  Statistics: for every GN_FOLD pixels a
+// lane sums x - k and (x - k)^2 with k the first of these values -- k is one of the values, so (k - mean)^2 <= M2 and the difference
+// sum (x-k)^2 - (sum (x-k))^2 / n loses at most a factor GN_FOLD + 1, whatever the mean.  Means and centred sums
+// (M2 = sum (x - mean)^2) are then joined as  mean = sum n_i mean_i / n,  M2 = sum M2_i + n_i (mean_i - mean)^2, always in the same
+// order: two runs give the same bits.  No chain of float additions is longer than GN_FOLD + GN_MOST: a lane folds its sums every GN_FOLD
+// pixels and has at most GN_FOLD * GN_MOST of them, the sums over chunks are in double.
 //
 // Measured on one MI355X, whose copy of 1 GiB reaches 5.2 TB/s.  Streaming form, 16 images of 128 x 224 x 64 bfloat16 with ReLU: sums
 // 15.0 us (3.9 TB/s), joining 4.0, applying 24.4 (4.8 TB/s, part of its reads from the caches).  One-launch form, 16 images of
@@ -22,6 +23,8 @@
 #define GN_MAXOCT 64           // octets of a workgroup: 512 channels
 #define GN_U 4                 // pixels of a lane in flight, forward
 #define GN_UB 2                // ... and backward (two tensors)
+#define GN_FOLD 64             // pixels of a lane whose sums are added up before they are joined with its others
+#define GN_MOST 64             // such runs of a lane
 
 // Activations in three classes, so that a kernel holds the code of one and no branch per element:
 //   0  max(z, 0) + p0 min(z, 0): none (1), ReLU (0), LeakyReLU (0.1)
@@ -135,18 +138,22 @@ template <typename T, bool AL> __global__ __launch_bounds__(GN_BLOCK) void gn_pa
     const long long p0 = (long long)chunk * a.per;
     const long long p1 = p0 + a.per < a.HW ? p0 + a.per : a.HW;
     const T* x = (const T*)a.x + (long long)n * a.HW * a.ldx + c0;
-    float k[8], s[8], q[8], cnt = 0.f;
+    float mean[8], m2[8], tot[8], cnt = 0.f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) k[e] = s[e] = q[e] = 0.f;
-    if (nv > 0 && p0 + pl < p1) {
-        load8<T, AL>(x + (p0 + pl) * a.ldx, nv, k);
-        for (long long p = p0 + pl; p < p1; p += U * lanes) {
+    for (int e = 0; e < 8; ++e) mean[e] = m2[e] = 0.f;
+    for (long long b = p0 + pl; nv > 0 && b < p1; b += GN_FOLD * lanes) {
+        const long long b1 = b + GN_FOLD * lanes < p1 ? b + GN_FOLD * lanes : p1;
+        float k[8], s[8], q[8], n = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[e] = q[e] = 0.f;
+        load8<T, AL>(x + b * a.ldx, nv, k);
+        for (long long p = b; p < b1; p += U * lanes) {
             float v[U][8];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const long long r = p + u * lanes;
-                load8<T, AL>(x + (r < p1 ? r : p0 + pl) * a.ldx, nv, v[u]);        // (past the end: the pivot again, difference 0)
-                cnt += r < p1 ? 1.f : 0.f;
+                load8<T, AL>(x + (r < b1 ? r : b) * a.ldx, nv, v[u]);              // (past the end: the pivot again, difference 0)
+                n += r < b1 ? 1.f : 0.f;
             }
 #pragma unroll
             for (int u = 0; u < U; ++u)
@@ -157,16 +164,25 @@ template <typename T, bool AL> __global__ __launch_bounds__(GN_BLOCK) void gn_pa
                     q[e] = fmaf(d, d, q[e]);
                 }
         }
-    }
-    float mean[8], m2[8], tot[8];
-    const float ic = cnt > 0.f ? 1.f / cnt : 0.f;
+        const float in = 1.f / n, f = n / (cnt + n);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        m2[e] = fmaxf(q[e] - s[e] * s[e] * ic, 0.f);
-        if (q[e] != q[e]) m2[e] = q[e];
-        mean[e] = k[e] + s[e] * ic;
-        tot[e] = mean[e] * cnt;
+        for (int e = 0; e < 8; ++e) {
+            float c2 = fmaxf(q[e] - s[e] * s[e] * in, 0.f);
+            if (q[e] != q[e]) c2 = q[e];
+            const float c1 = k[e] + s[e] * in;
+            if (cnt == 0.f) {
+                mean[e] = c1;
+                m2[e] = c2;
+            } else {
+                const float d = c1 - mean[e];
+                mean[e] = fmaf(d, f, mean[e]);
+                m2[e] += fmaf(d * d, cnt * f, c2);
+            }
+        }
+        cnt += n;
     }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) tot[e] = mean[e] * cnt;
     gn_reduce(tot, a.octp, red);
     const float in = 1.f / (float)(p1 - p0);
 #pragma unroll
@@ -301,24 +317,35 @@ template <typename T, bool AL, int CLS> __global__ __launch_bounds__(GN_BLOCK) v
         gn_channels(a, n, c0, nv, ch);
         const T* x = (const T*)a.x + (long long)n * a.HW * a.ldx + c0;
         const T* dy = (const T*)a.dy + (long long)n * a.HW * a.lddy + c0;
-        for (long long p = p0 + pl; p < p1; p += GN_UB * lanes) {
-            float v[GN_UB][8], d[GN_UB][8];
+        for (long long b = p0 + pl; b < p1; b += GN_FOLD * lanes) {
+            const long long b1 = b + GN_FOLD * lanes < p1 ? b + GN_FOLD * lanes : p1;
+            float sb[8], qb[8];
 #pragma unroll
-            for (int u = 0; u < GN_UB; ++u)
-                if (p + u * lanes < p1) {
-                    load8<T, AL>(x + (p + u * lanes) * a.ldx, nv, v[u]);
-                    load8<T, AL>(dy + (p + u * lanes) * a.lddy, nv, d[u]);
-                }
+            for (int e = 0; e < 8; ++e) sb[e] = qb[e] = 0.f;
+            for (long long p = b; p < b1; p += GN_UB * lanes) {
+                float v[GN_UB][8], d[GN_UB][8];
 #pragma unroll
-            for (int u = 0; u < GN_UB; ++u)
-                if (p + u * lanes < p1)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const float x0 = v[u][e] - ch.mean[e];
-                        const float dz = d[u][e] * gn_slope<T, CLS>(fmaf(x0, ch.k[e], ch.be[e]), a.act);
-                        s[e] += dz;
-                        q[e] = fmaf(dz, x0, q[e]);
+                for (int u = 0; u < GN_UB; ++u)
+                    if (p + u * lanes < b1) {
+                        load8<T, AL>(x + (p + u * lanes) * a.ldx, nv, v[u]);
+                        load8<T, AL>(dy + (p + u * lanes) * a.lddy, nv, d[u]);
                     }
+#pragma unroll
+                for (int u = 0; u < GN_UB; ++u)
+                    if (p + u * lanes < b1)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const float x0 = v[u][e] - ch.mean[e];
+                            const float dz = d[u][e] * gn_slope<T, CLS>(fmaf(x0, ch.k[e], ch.be[e]), a.act);
+                            sb[e] += dz;
+                            qb[e] = fmaf(dz, x0, qb[e]);
+                        }
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                s[e] += sb[e];
+                q[e] += qb[e];
+            }
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) q[e] *= ch.rstd[e];

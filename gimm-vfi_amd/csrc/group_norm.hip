@@ -1,90 +1,95 @@
 // Group norm with an activation: the C ABI, the kernels without an element type, the choice of form (group_norm.h has the rest).
 #include "group_norm.h"
 
-// sum over the workgroup, in every lane
-__device__ __forceinline__ float gn_block_sum(float v, float* red) {
-    v = wave_sum(v);
+// sum over the workgroup, in every lane, in double
+__device__ __forceinline__ double gn_block_sum(double v, double* red) {
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    red[threadIdx.x] = v;
     __syncthreads();
-    float s = 0.f;
+    if (threadIdx.x < 16) {
+        v = 0.0;
 #pragma unroll
-    for (int k = 0; k < GN_BLOCK / 64; ++k) s += red[k];
-    return s;
+        for (int k = 0; k < GN_BLOCK / 16; ++k) v += red[threadIdx.x + 16 * k];
+        red[threadIdx.x] = v;
+    }
+    __syncthreads();
+    v = 0.0;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) v += red[k];
+    return v;
 }
 
 // joins the chunks of a group, and its channels where they come one by one (cols = C values per chunk, `per_group` of them a group's)
 __global__ __launch_bounds__(GN_BLOCK) void gn_stats_kernel(const float* part, float* stats, long long HW, long long per, int cols,
                                                             int G, int per_group, int Cg, int chunks, float eps) {
-    __shared__ float red[GN_BLOCK / 64];
+    __shared__ double red[GN_BLOCK];
     const int n = blockIdx.x / G, g = blockIdx.x - n * G;
     const float* w = part + (long long)n * chunks * 2 * cols + g * per_group;
     const long long items = (long long)chunks * per_group;
-    const float share = (float)(Cg / per_group);             // values of a pixel in an item
-    float s = 0.f;
+    const double share = (double)(Cg / per_group);           // values of a pixel in an item
+    double s = 0.0;
     for (long long i = threadIdx.x; i < items; i += GN_BLOCK) {
         const long long k = per_group == 1 ? i : i / per_group;
-        const float cnt = share * (float)(k + 1 < chunks ? per : HW - k * per);
-        s += cnt * w[k * 2 * cols + (i - k * per_group)];
+        const double cnt = share * (double)(k + 1 < chunks ? per : HW - k * per);
+        s += cnt * (double)w[k * 2 * cols + (i - k * per_group)];
     }
-    const float m = (float)HW * (float)Cg;
-    const float mean = gn_block_sum(s, red) / m;
-    float q = 0.f;
+    const double m = (double)HW * (double)Cg;
+    const double mean = gn_block_sum(s, red) / m;
+    double q = 0.0;
     for (long long i = threadIdx.x; i < items; i += GN_BLOCK) {
         const long long k = per_group == 1 ? i : i / per_group;
-        const float cnt = share * (float)(k + 1 < chunks ? per : HW - k * per);
-        const float d = w[k * 2 * cols + (i - k * per_group)] - mean;
-        q += w[(k * 2 + 1) * cols + (i - k * per_group)] + cnt * d * d;
+        const double cnt = share * (double)(k + 1 < chunks ? per : HW - k * per);
+        const double d = (double)w[k * 2 * cols + (i - k * per_group)] - mean;
+        q += (double)w[(k * 2 + 1) * cols + (i - k * per_group)] + cnt * d * d;
     }
-    const float var = gn_block_sum(q, red) / m;
+    const float var = (float)(gn_block_sum(q, red) / m);
     if (threadIdx.x == 0) {
-        stats[((long long)n * G + g) * 2] = mean;
+        stats[((long long)n * G + g) * 2] = (float)mean;
         stats[((long long)n * G + g) * 2 + 1] = 1.f / sqrtf(var + eps);
     }
 }
 
 // sums of an image's channels over its chunks, and A, B of the group
 __global__ __launch_bounds__(GN_BLOCK) void gn_bwd_group_kernel(GnArgs a) {
-    __shared__ float red[GN_BLOCK / 64];
-    __shared__ float sh[2][GN_BLOCK];
+    __shared__ double sh[2][GN_BLOCK];
     const int n = blockIdx.x / a.G, g = blockIdx.x - n * a.G;
     int cp = 1;                                     // channels side by side, the chunks in GN_BLOCK / cp parts
     while (cp < a.Cg && cp < GN_BLOCK) cp <<= 1;
     const int cl = threadIdx.x & (cp - 1), part = threadIdx.x / cp, parts = GN_BLOCK / cp;
     const float* w = a.part + (long long)n * a.chunks * 2 * a.C + g * a.Cg;
-    float ga = 0.f, gb = 0.f;
+    double ga = 0.0, gb = 0.0;
     for (int cb = 0; cb < a.Cg; cb += cp) {
         const int c = cb + cl;
-        float s = 0.f, q = 0.f;
+        double s = 0.0, q = 0.0;
         if (c < a.Cg)
             for (int k = part; k < a.chunks; k += parts) {
-                s += w[(long long)k * 2 * a.C + c];
-                q += w[((long long)k * 2 + 1) * a.C + c];
+                s += (double)w[(long long)k * 2 * a.C + c];
+                q += (double)w[((long long)k * 2 + 1) * a.C + c];
             }
         __syncthreads();
         sh[0][threadIdx.x] = s;
         sh[1][threadIdx.x] = q;
         __syncthreads();
         if (part == 0 && c < a.Cg) {
-            s = q = 0.f;
+            s = q = 0.0;
             for (int k = 0; k < parts; ++k) {
                 s += sh[0][k * cp + cl];
                 q += sh[1][k * cp + cl];
             }
             const int cc = g * a.Cg + c;
-            a.sums[(long long)n * 2 * a.C + cc] = s;
-            a.sums[((long long)n * 2 + 1) * a.C + cc] = q;
-            const float gm = a.gamma ? a.gamma[cc] : 1.f;
+            a.sums[(long long)n * 2 * a.C + cc] = (float)s;
+            a.sums[((long long)n * 2 + 1) * a.C + cc] = (float)q;
+            const double gm = a.gamma ? (double)a.gamma[cc] : 1.0;
             ga += gm * s;
             gb += gm * q;
         }
     }
-    ga = gn_block_sum(ga, red);
-    gb = gn_block_sum(gb, red);
+    ga = gn_block_sum(ga, sh[0]);
+    gb = gn_block_sum(gb, sh[1]);
     if (threadIdx.x == 0) {
-        const float m = (float)a.HW * (float)a.Cg;
-        a.ab[((long long)n * a.G + g) * 2] = ga / m;
-        a.ab[((long long)n * a.G + g) * 2 + 1] = gb / m;
+        const double m = (double)a.HW * (double)a.Cg;
+        a.ab[((long long)n * a.G + g) * 2] = (float)(ga / m);
+        a.ab[((long long)n * a.G + g) * 2 + 1] = (float)(gb / m);
     }
 }
 
@@ -123,8 +128,12 @@ static int gn_check(int C, int G, long long N, long long HW, int act, int dtype)
     return 0;
 }
 // Pixels per workgroup: as many workgroups as the CUs hold at once (five of the applying kernels on each; a second round for the rest
-// costs more than a longer first one), at least two octets per lane
+// costs more than a longer first one), at least two octets per lane and at most GN_FOLD * GN_MOST
+#ifndef GVFI_HOSTSIM
 #define GN_WORKGROUPS 1280
+#else
+#define GN_WORKGROUPS 16        // (the emulator's tests reach long chunks)
+#endif
 static bool gn_plan(GnArgs& a) {
     const int oct = (a.C + 7) / 8, o = oct < GN_MAXOCT ? oct : GN_MAXOCT;
     a.octp = 1;
@@ -134,8 +143,11 @@ static bool gn_plan(GnArgs& a) {
     long long want = (GN_WORKGROUPS + images - 1) / images;                       // chunks of an image
     long long per = (a.HW + want - 1) / want;
     if (per < lanes * 2) per = lanes * 2;
+    if (per > lanes * GN_FOLD * GN_MOST) per = lanes * GN_FOLD * GN_MOST;
     a.per = (per + lanes - 1) / lanes * lanes;
-    a.chunks = (int)((a.HW + a.per - 1) / a.per);
+    const long long chunks = (a.HW + a.per - 1) / a.per;
+    if (chunks >= (1LL << 23)) return false;
+    a.chunks = (int)chunks;
     a.whole = a.C <= GN_MAXOCT * 8 || GN_MAXOCT * 8 % (a.C / a.G) == 0;
     // (a launch has fewer than 2^32 lanes: 2^23 workgroups of 512, the images of the one-launch form rounded up to eights; 2^24 of 256
     // in gn_params)

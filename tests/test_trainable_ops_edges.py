@@ -5,6 +5,7 @@ import pytest
 import torch
 
 import train_ops_oracle as orc
+from gimmvfi_hip import group_norm as gn
 from gimmvfi_hip import lib as L
 from gimmvfi_hip import rel_softmax as rs
 from test_trainable_ops import BF16, F16, F32, _gen, _rs_case, _rs_plan, _runtime, _within, dev  # noqa: F401
@@ -112,3 +113,48 @@ def test_gpu_softmax_rel_bias_one_query_2_28_keys():
     dot = (p * g).sum()
     tol = p * (rel * (g - dot).abs() + (p * g.abs()).sum() * (rel + 96 * orc.U) + 8 * orc.U * (g.abs() + dot.abs())) + 2.0 ** -126
     assert bool(((dx.view(-1).double() - p * (g - dot)).abs() <= tol + 2 * orc.U * (p * (g - dot)).abs()).all())
+
+
+# ------------------------------------------------------------------------------------------------ long sums
+def _statistics(x, dy, groups, eps=1e-5):
+    """64-bit mean, rstd of the groups, sum dy and sum dy xhat of the channels (no activation, no weights) of x, dy (N, P, C), with bounds as
+    in train_ops_oracle.group_norm: 64 roundings of the mean, 72 of xhat, 96 of a channel's sums.  By runs of pixels: x may be large."""
+    n, p, c = x.shape
+    cg = c // groups
+    runs = range(0, p, 1 << 15)
+    tot = torch.zeros(n, groups, dtype=torch.float64, device=x.device)
+    mag = torch.zeros_like(tot)
+    for r in runs:
+        v = x[:, r:r + (1 << 15)].double().reshape(n, -1, groups, cg)
+        tot += v.sum((1, 3))
+        mag += v.abs().sum((1, 3))
+    mean, mag = tot / (p * cg), mag / (p * cg)
+    sq = torch.zeros_like(tot)
+    for r in runs:
+        sq += ((x[:, r:r + (1 << 15)].double().reshape(n, -1, groups, cg) - mean.view(n, 1, groups, 1)) ** 2).sum((1, 3))
+    rstd = 1 / torch.sqrt(sq / (p * cg) + eps)
+    sums = [torch.zeros(c, dtype=torch.float64, device=x.device) for _ in range(4)]
+    for r in runs:
+        v = x[:, r:r + (1 << 15)].double().reshape(n, -1, groups, cg)
+        d = dy[:, r:r + (1 << 15)].double().reshape(v.shape)
+        hat = (v - mean.view(n, 1, groups, 1)) * rstd.view(n, 1, groups, 1)
+        h_err = orc.U * (64 * ((mag + mean.abs()).view(n, 1, groups, 1) + v.abs()) * rstd.view(n, 1, groups, 1) + 72 * hat.abs())
+        for s, t in zip(sums, (d, 96 * orc.U * d.abs(), d * hat, d.abs() * h_err + 96 * orc.U * (d * hat).abs())):
+            s += t.sum((0, 1)).reshape(c)
+    return (mean, 64 * orc.U * (mag + mean.abs())), (rstd, 72 * orc.U * rstd), sums[:2], sums[2:]
+
+
+def test_group_norm_sums_of_many_pixels_per_lane(dev):
+    """400 pixels for each of the four lanes of an octet of 512 channels, the first values so large that a chain of additions behind them
+    loses every one: a lane's sums have to be folded on the way."""
+    p = (16 if dev.type == "cpu" else 1280) * 4 * 400
+    i = torch.arange(p, device=dev) // 4 % 400
+    x = torch.where(i == 0, 0.0, torch.where(i == 1, 2.0 ** 24, 1.0)).to(BF16).view(1, p, 1).expand(1, p, 512).contiguous()
+    dy = torch.where(i == 0, 2.0 ** 24, 1.0).to(BF16).view(1, p, 1).expand(1, p, 512).contiguous()
+    mean, rstd, db, dw = _statistics(x, dy, 1)
+    y, stats = gn.forward(x, 1)
+    _within(stats[..., 0], *mean, "mean")
+    _within(stats[..., 1], *rstd, "rstd")
+    _, dgamma, dbeta = gn.backward(dy, x, stats, 1)
+    _within(dbeta, *db, "dbias")
+    _within(dgamma, *dw, "dweight")
