@@ -443,7 +443,9 @@ template <typename TX, typename TY, int PHASE> __global__ __launch_bounds__(512)
     }
     const float top = m == -INFINITY ? 0.f : m;
     if (PHASE == 1) {
-        for (int k = 0; k < a.tiles; ++k) s += part[2 * k + 1] * rs_exp(part[2 * k] - top);
+        double all = 0.0;                                    // (a row may have 2^17 tiles)
+        for (int k = 0; k < a.tiles; ++k) all += (double)(part[2 * k + 1] * rs_exp(part[2 * k] - top));
+        s = (float)all;
         inv = s == 0.f ? 0.f : 1.f / s;
         TY* y = (TY*)a.y + r * a.ldy;
 #pragma unroll
@@ -559,8 +561,9 @@ __global__ __launch_bounds__(T < 64 ? RS_BLOCK : T) void rs_backward_kernel(RsAr
             }
         }
         if (SPLIT && PHASE == 1) {
-            dot[0] = 0.f;
-            for (int w = 0; w < a.tiles; ++w) dot[0] += a.part[row[0] * a.tiles + w];
+            double all = 0.0;
+            for (int w = 0; w < a.tiles; ++w) all += (double)a.part[row[0] * a.tiles + w];
+            dot[0] = (float)all;
             if (adds) __syncthreads();
         } else {
 #pragma unroll

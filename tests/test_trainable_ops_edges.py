@@ -1,6 +1,8 @@
 """Edges of group norm, dropout and the biased row soft-max: arguments that do not fit the launch, values at the ends of the types'
 ranges, long sums.  As in test_trainable_ops.py the kernel sources run in the host emulator on the CPU and as the gfx950 library with
 ``-m gpu``."""
+import math
+
 import pytest
 import torch
 
@@ -158,3 +160,21 @@ def test_group_norm_sums_of_many_pixels_per_lane(dev):
     _, dgamma, dbeta = gn.backward(dy, x, stats, 1)
     _within(dbeta, *db, "dbias")
     _within(dgamma, *dw, "dweight")
+
+
+def test_softmax_rel_bias_sums_of_many_tiles(dev):
+    """A row in 200 tiles of 8192 columns.  The first tile's sum is 1, every other tile adds 0.12 steps of float to it (2^-23 each): additions
+    one behind the other in float would lose them all, 24 steps together."""
+    m = 200 * 8192
+    x = torch.full((m,), -15.9423851 - math.log(8192.0) + math.log(0.12))
+    x[0] = 0.0
+    x[1:8192] = -math.inf
+    e = torch.exp(x.double())
+    plan = rs.RelativeBuckets((1, 1), (1, m), torch.zeros(1, m, dtype=torch.int64, device=dev), 1)
+    table = torch.zeros(1, 1, device=dev)
+    y, stats = rs.forward(x.view(1, 1, 1, m).to(dev), table, plan)
+    # 1 / sum: at most 16 roundings in a tile, the joined sum's and the inverse's, of terms that are all positive; the exponential's own
+    # error (|x| / 2 steps and one) applies to the small part of the sum only
+    small = float(e.sum()) - 1.0
+    tol = 2.0 * orc.U + small * 64 * orc.U
+    assert abs(float(stats[0, 0, 0, 1]) * float(e.sum()) - 1.0) <= tol, (float(stats[0, 0, 0, 1]), float(e.sum()))
