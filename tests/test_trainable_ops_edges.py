@@ -10,7 +10,7 @@ import train_ops_oracle as orc
 from gimmvfi_hip import group_norm as gn
 from gimmvfi_hip import lib as L
 from gimmvfi_hip import rel_softmax as rs
-from test_trainable_ops import BF16, F16, F32, _gen, _rs_case, _rs_plan, _runtime, _within, dev  # noqa: F401
+from test_trainable_ops import BF16, F16, F32, _gen, _gn_case, _gn_inputs, _rs_case, _rs_inputs, _rs_plan, _runtime, _within, dev  # noqa: F401
 
 
 # ------------------------------------------------------------------------------------------------ the launch list's arguments
@@ -178,3 +178,78 @@ def test_softmax_rel_bias_sums_of_many_tiles(dev):
     small = float(e.sum()) - 1.0
     tol = 2.0 * orc.U + small * 64 * orc.U
     assert abs(float(stats[0, 0, 0, 1]) * float(e.sum()) - 1.0) <= tol, (float(stats[0, 0, 0, 1]), float(e.sum()))
+
+
+# a mean far above the spread: the one-launch form, streaming with octets that are not whole, streaming with aligned octets, channels one by
+# one (more than a workgroup covers, groups that do not fit it)
+@pytest.mark.parametrize("shape,groups", [((2, 99, 16), 2), ((2, 2000, 12), 3), ((1, 1100, 16), 1), ((1, 70, 1032), 3)],
+                         ids=lambda v: str(v).replace(" ", ""))
+def test_group_norm_common_mean_of_a_thousand(dev, shape, groups):
+    g = _gen(7)
+    x, dy = torch.randn(shape, generator=g) + 1000.0, torch.randn(shape, generator=g)
+    ref = orc.group_norm(x, groups, None, None, L.ACT_NONE, 1e-5, dy)
+    # the difference of the mean square and the squared mean, in float, is not good enough for these bounds
+    v = x.reshape(shape[0], -1, groups, shape[-1] // groups)
+    mean, sq = v.mean((1, 3), keepdim=True), (v * v).mean((1, 3), keepdim=True)
+    naive = ((v - mean) / torch.sqrt(torch.clamp(sq - mean * mean, min=0) + 1e-5)).reshape(shape)
+    assert bool(((naive.double() - ref["y"]).abs() > ref["y_tol"]).any())
+    y, stats = gn.forward(x.to(dev), groups)
+    _within(y, ref["y"], ref["y_tol"], "y")
+    dx, dw, db = gn.backward(dy.to(dev), x.to(dev), stats, groups)
+    for got, k in ((dx, "dx"), (dw, "dw"), (db, "db")):
+        _within(got, ref[k], ref[k + "_tol"], k)
+
+
+# forms that the cases of test_trainable_ops.py do not reach in the emulator: aligned octets streamed in several chunks; the parameters'
+# gradients of more than 128 images behind the streaming form
+@pytest.mark.parametrize("case", [((1, 1100, 16), 1, L.ACT_SILU, F32, None, 0, True), ((3, 700, 64), 4, L.ACT_GELU, BF16, 72, 8, True),
+                                  ((130, 3, 256), 1, L.ACT_GELU, BF16, None, 0, True), ((131, 5, 20), 5, L.ACT_TANH, F16, 23, 1, True),
+                                  ((260, 2, 136), 1, L.ACT_SIGMOID, F32, None, 0, True)],
+                         ids=lambda c: f"{'x'.join(map(str, c[0]))}-{c[1]}-{str(c[3])[6:]}")
+def test_group_norm_streamed(dev, case):
+    _gn_case(dev, *case)
+
+
+# ------------------------------------------------------------------------------------------------ offsets beyond 32 bits
+@pytest.mark.gpu
+def test_gpu_group_norm_pitched_rows_beyond_32_bits_of_elements():
+    """Two images of 40000 pixels of 24 channels at a pitch of 32768: the second lies behind 2^30 elements, its last pixels behind 2^31."""
+    d = torch.device("cuda", 0)
+    x, w, b, dy = _gn_inputs((2, 40000, 24), BF16, 12)
+    wide = [torch.full((2, 40000, 32768), float("nan"), dtype=BF16, device=d) for _ in range(2)]
+    assert wide[0].numel() > 1 << 31
+    for t, v in zip(wide, (x, dy)):
+        t[..., 32000:32024] = v.to(d)
+    xd, dyd = (t[..., 32000:32024] for t in wide)
+    ref = orc.group_norm(x, 3, w, b, L.ACT_SILU, 1e-5, dy)
+    y, stats = gn.forward(xd, 3, w.to(d), b.to(d), L.ACT_SILU, out=wide[0][..., 8:32])
+    _within(y, ref["y"], ref["y_tol"], "y")
+    dx, dw, db = gn.backward(dyd, xd, stats, 3, w.to(d), b.to(d), L.ACT_SILU)
+    for got, k in ((dx, "dx"), (dw, "dw"), (db, "db")):
+        _within(got, ref[k], ref[k + "_tol"], k)
+    assert bool(wide[0][..., 32:32000].isnan().all()) and bool(wide[0][..., :8].isnan().all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", [(4, 1, (7, 7), (7, 7), "grid", 13_000_000), (2, 1, (5, 8), (13, 20), "grid", 30_000_000),
+                                  (2, 1, (5, 4), (13, 11), "shared", 60_000_000), (1, 1, (1, 110), (1, 20000), "log", 20_000_000)],
+                         ids=lambda c: f"{c[2]}-{c[3]}-{c[4]}")
+def test_gpu_softmax_rel_bias_pitched_rows_beyond_32_bits_of_elements(case):
+    """Every form of the kernels with the last rows behind 2^31 elements, scores, gradients and probabilities alike."""
+    d = torch.device("cuda", 0)
+    B, heads, q, k, kind, pitch = case
+    plan, x, table, mask, dy = _rs_inputs(B, heads, q, k, kind, BF16, BF16, False, d)
+    n, m = x.numel() // x.shape[-1], x.shape[-1]
+    assert (n - 1) * pitch > 1 << 31
+    ref = orc.softmax_rel_bias(x, table, plan.bucket_of, q, k, 0.7, None, BF16, dy)
+    def spread(t):
+        wide = torch.empty(n * pitch, dtype=BF16, device=d).as_strided(x.shape, (heads * x.shape[2] * pitch, x.shape[2] * pitch, pitch, 1))
+        wide.copy_(t)
+        return wide
+    xd, dyd, td = spread(x), spread(dy), table.to(d)
+    y, stats = rs.forward(xd, td, plan, 0.7, pitch=pitch)
+    _within(y, ref["y"], ref["y_tol"], "y")
+    del y
+    dx, dt = rs.backward(dyd, xd, stats, td, plan, 0.7)
+    _within(dx, ref["dx"], ref["dx_tol"], "dx")
+    _within(dt, ref["dtable"], ref["dtable_tol"], "dtable")
