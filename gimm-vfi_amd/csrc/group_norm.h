@@ -131,6 +131,7 @@ __device__ __forceinline__ void gn_reduce(float (&v)[8], int octp, float* red) {
 template <typename T, bool AL> __global__ __launch_bounds__(GN_BLOCK) void gn_partial_kernel(GnArgs a) {
     constexpr int U = GN_U;
     __shared__ float red[GN_BLOCK / 64 * GN_MAXOCT * 8];
+    __shared__ float kept[16][GN_BLOCK];           // what a lane has joined so far: mean, M2 (in registers they would cost a third of the waves)
     const int o = threadIdx.x & (a.octp - 1), pl = threadIdx.x / a.octp, lanes = GN_BLOCK / a.octp;
     const int c0 = (blockIdx.y * GN_MAXOCT + o) * 8;
     const int nv = a.C - c0 < 8 ? a.C - c0 : 8;
@@ -138,22 +139,36 @@ template <typename T, bool AL> __global__ __launch_bounds__(GN_BLOCK) void gn_pa
     const long long p0 = (long long)chunk * a.per;
     const long long p1 = p0 + a.per < a.HW ? p0 + a.per : a.HW;
     const T* x = (const T*)a.x + (long long)n * a.HW * a.ldx + c0;
-    float mean[8], m2[8], tot[8], cnt = 0.f;
+    float k[8], s[8], q[8], mean[8], m2[8], tot[8], n1 = 0.f, cnt = 0.f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) mean[e] = m2[e] = 0.f;
-    for (long long b = p0 + pl; nv > 0 && b < p1; b += GN_FOLD * lanes) {
-        const long long b1 = b + GN_FOLD * lanes < p1 ? b + GN_FOLD * lanes : p1;
-        float k[8], s[8], q[8], n = 0.f;
+    for (int e = 0; e < 8; ++e) k[e] = s[e] = q[e] = 0.f;
+    // joins the sums (s, q) of n1 pixels to what `kept` has of cnt pixels
+    auto join = [&]() {
+        const float in = n1 > 0.f ? 1.f / n1 : 0.f, f = n1 / (cnt + n1);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) s[e] = q[e] = 0.f;
-        load8<T, AL>(x + b * a.ldx, nv, k);
-        for (long long p = b; p < b1; p += U * lanes) {
+        for (int e = 0; e < 8; ++e) {
+            m2[e] = fmaxf(q[e] - s[e] * s[e] * in, 0.f);
+            if (q[e] != q[e]) m2[e] = q[e];
+            mean[e] = k[e] + s[e] * in;
+            if (cnt > 0.f) {
+                const float mk = kept[e][threadIdx.x], d = mean[e] - mk;
+                mean[e] = n1 > 0.f ? fmaf(d, f, mk) : mk;
+                m2[e] = kept[8 + e][threadIdx.x] + (n1 > 0.f ? fmaf(d * d, cnt * f, m2[e]) : 0.f);
+            }
+        }
+        cnt += n1;
+    };
+    if (nv > 0 && p0 + pl < p1) {
+        long long pivot = p0 + pl;
+        load8<T, AL>(x + pivot * a.ldx, nv, k);
+        int turns = 0;
+        for (long long p = p0 + pl; p < p1; p += U * lanes) {
             float v[U][8];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const long long r = p + u * lanes;
-                load8<T, AL>(x + (r < b1 ? r : b) * a.ldx, nv, v[u]);              // (past the end: the pivot again, difference 0)
-                n += r < b1 ? 1.f : 0.f;
+                load8<T, AL>(x + (r < p1 ? r : pivot) * a.ldx, nv, v[u]);          // (past the end: the pivot again, difference 0)
+                n1 += r < p1 ? 1.f : 0.f;
             }
 #pragma unroll
             for (int u = 0; u < U; ++u)
@@ -163,24 +178,24 @@ template <typename T, bool AL> __global__ __launch_bounds__(GN_BLOCK) void gn_pa
                     s[e] += d;
                     q[e] = fmaf(d, d, q[e]);
                 }
-        }
-        const float in = 1.f / n, f = n / (cnt + n);
+            if (++turns == GN_FOLD / U) {
+                join();
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            float c2 = fmaxf(q[e] - s[e] * s[e] * in, 0.f);
-            if (q[e] != q[e]) c2 = q[e];
-            const float c1 = k[e] + s[e] * in;
-            if (cnt == 0.f) {
-                mean[e] = c1;
-                m2[e] = c2;
-            } else {
-                const float d = c1 - mean[e];
-                mean[e] = fmaf(d, f, mean[e]);
-                m2[e] += fmaf(d * d, cnt * f, c2);
+                for (int e = 0; e < 8; ++e) {
+                    kept[e][threadIdx.x] = mean[e];
+                    kept[8 + e][threadIdx.x] = m2[e];
+                    s[e] = q[e] = 0.f;
+                }
+                n1 = 0.f;
+                turns = 0;
+                if (p + U * lanes < p1) {
+                    pivot = p + U * lanes;
+                    load8<T, AL>(x + pivot * a.ldx, nv, k);
+                }
             }
         }
-        cnt += n;
     }
+    join();
 #pragma unroll
     for (int e = 0; e < 8; ++e) tot[e] = mean[e] * cnt;
     gn_reduce(tot, a.octp, red);
@@ -303,6 +318,7 @@ template <typename T, bool AL, int CLS> __global__ __launch_bounds__(GN_BLOCK) v
 // ---- backward
 template <typename T, bool AL, int CLS> __global__ __launch_bounds__(GN_BLOCK) void gn_bwd_partial_kernel(GnArgs a) {
     __shared__ float red[GN_BLOCK / 64 * GN_MAXOCT * 8];
+    __shared__ float kept[16][GN_BLOCK];           // a lane's sums of the pixels before the last GN_FOLD
     const int o = threadIdx.x & (a.octp - 1), pl = threadIdx.x / a.octp, lanes = GN_BLOCK / a.octp;
     const int c0 = (blockIdx.y * GN_MAXOCT + o) * 8;
     const int nv = a.C - c0 < 8 ? a.C - c0 : 8;
@@ -317,36 +333,43 @@ template <typename T, bool AL, int CLS> __global__ __launch_bounds__(GN_BLOCK) v
         gn_channels(a, n, c0, nv, ch);
         const T* x = (const T*)a.x + (long long)n * a.HW * a.ldx + c0;
         const T* dy = (const T*)a.dy + (long long)n * a.HW * a.lddy + c0;
-        for (long long b = p0 + pl; b < p1; b += GN_FOLD * lanes) {
-            const long long b1 = b + GN_FOLD * lanes < p1 ? b + GN_FOLD * lanes : p1;
-            float sb[8], qb[8];
+        int turns = 0;
+        bool folded = false;
+        for (long long p = p0 + pl; p < p1; p += GN_UB * lanes) {
+            float v[GN_UB][8], d[GN_UB][8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) sb[e] = qb[e] = 0.f;
-            for (long long p = b; p < b1; p += GN_UB * lanes) {
-                float v[GN_UB][8], d[GN_UB][8];
+            for (int u = 0; u < GN_UB; ++u)
+                if (p + u * lanes < p1) {
+                    load8<T, AL>(x + (p + u * lanes) * a.ldx, nv, v[u]);
+                    load8<T, AL>(dy + (p + u * lanes) * a.lddy, nv, d[u]);
+                }
 #pragma unroll
-                for (int u = 0; u < GN_UB; ++u)
-                    if (p + u * lanes < b1) {
-                        load8<T, AL>(x + (p + u * lanes) * a.ldx, nv, v[u]);
-                        load8<T, AL>(dy + (p + u * lanes) * a.lddy, nv, d[u]);
+            for (int u = 0; u < GN_UB; ++u)
+                if (p + u * lanes < p1)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float x0 = v[u][e] - ch.mean[e];
+                        const float dz = d[u][e] * gn_slope<T, CLS>(fmaf(x0, ch.k[e], ch.be[e]), a.act);
+                        s[e] += dz;
+                        q[e] = fmaf(dz, x0, q[e]);
                     }
+            if (++turns == GN_FOLD / GN_UB) {
 #pragma unroll
-                for (int u = 0; u < GN_UB; ++u)
-                    if (p + u * lanes < b1)
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            const float x0 = v[u][e] - ch.mean[e];
-                            const float dz = d[u][e] * gn_slope<T, CLS>(fmaf(x0, ch.k[e], ch.be[e]), a.act);
-                            sb[e] += dz;
-                            qb[e] = fmaf(dz, x0, qb[e]);
-                        }
-            }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                s[e] += sb[e];
-                q[e] += qb[e];
+                for (int e = 0; e < 8; ++e) {
+                    kept[e][threadIdx.x] = folded ? kept[e][threadIdx.x] + s[e] : s[e];
+                    kept[8 + e][threadIdx.x] = folded ? kept[8 + e][threadIdx.x] + q[e] : q[e];
+                    s[e] = q[e] = 0.f;
+                }
+                turns = 0;
+                folded = true;
             }
         }
+        if (folded)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                s[e] += kept[e][threadIdx.x];
+                q[e] += kept[8 + e][threadIdx.x];
+            }
 #pragma unroll
         for (int e = 0; e < 8; ++e) q[e] *= ch.rstd[e];
     }
