@@ -26,69 +26,92 @@
 #define GN_FOLD 64             // pixels of a lane whose sums are added up before they are joined with its others
 #define GN_MOST 64             // such runs of a lane
 
-// Activations in three classes, so that a kernel holds the code of one and no branch per element:
+// Activations in four classes, so that a kernel holds the code of one and no branch per element:
 //   0  max(z, 0) + p0 min(z, 0): none (1), ReLU (0), LeakyReLU (0.1)
-//   1  s (p1 z + p2) + p3 with s = sigmoid(p0 z): SiLU, sigmoid, tanh = 2 sigmoid(2z) - 1
+//   1  sigmoid s(z), and SiLU = z s(z) (p0 = 1)
 //   2  GELU (erf)
-// Class 1 takes 2^t and 1 / x from the hardware: a few steps of float absolute, which the library's exact exponential and division give
-// at five times the instructions (the backward pass of a 16-bit tensor was bound by them).  GELU of 16-bit tensors takes erf by Abramowitz and Stegun 7.1.26 (error below 1.5e-7, a thousandth of half's step), whose
-// exponential is the one that the derivative needs; float tensors take erff.
-struct GnAct { int cls; float p0, p1, p2, p3; };
+//   3  tanh
+// Every value and derivative is accurate relative to itself, not to 1: a small tanh, a far tail of GELU or a saturated sigmoid's derivative
+// keeps its digits (but for a derivative's own zero crossing).  float tensors take the library's exponential, erfc, tanh and an exact
+// division: the value's error is a few steps.  Tensors of 16 bits take 2^t and 1 / x of the hardware and an erfc of this file, together below
+// 2^-16 of the value, where half's own rounding is up to 2^-11: the library's functions cost five times the instructions, which the
+// backward pass of a 16-bit tensor was bound by.
+struct GnAct { int cls; float p0; };
 static inline GnAct gn_act_of(int act) {
     switch (act) {
-        case GVFI_ACT_RELU: return {0, 0.f, 0.f, 0.f, 0.f};
-        case GVFI_ACT_LRELU: return {0, 0.1f, 0.f, 0.f, 0.f};
-        case GVFI_ACT_SIGMOID: return {1, 1.f, 0.f, 1.f, 0.f};
-        case GVFI_ACT_TANH: return {1, 2.f, 0.f, 2.f, -1.f};
-        case GVFI_ACT_SILU: return {1, 1.f, 1.f, 0.f, 0.f};
-        case GVFI_ACT_GELU: return {2, 0.f, 0.f, 0.f, 0.f};
-        default: return {0, 1.f, 0.f, 0.f, 0.f};
+        case GVFI_ACT_RELU: return {0, 0.f};
+        case GVFI_ACT_LRELU: return {0, 0.1f};
+        case GVFI_ACT_SIGMOID: return {1, 0.f};
+        case GVFI_ACT_SILU: return {1, 1.f};
+        case GVFI_ACT_GELU: return {2, 0.f};
+        case GVFI_ACT_TANH: return {3, 0.f};
+        default: return {0, 1.f};
     }
 }
-__device__ __forceinline__ float gn_rcp(float x) {
+// 1 / x and exp(-x) for tensors of type T
+template <typename T> __device__ __forceinline__ float gn_rcp(float x) {
 #ifndef GVFI_HOSTSIM
-    return __builtin_amdgcn_rcpf(x);
-#else
-    return 1.f / x;
+    if constexpr (sizeof(T) == 2) return __builtin_amdgcn_rcpf(x);
 #endif
+    return 1.f / x;
 }
-// 1 / (1 + exp(-z)).  The exponential is off by |z| / 2 steps relative to itself, the sigmoid by s (1 - s) |z| <= 0.23 of that.
-__device__ __forceinline__ float gn_sig(float z) { return gn_rcp(1.f + exp2_hw(z * -1.44269504f)); }
-// Phi(z) = (1 + erf(z / sqrt 2)) / 2 and phi(z) = exp(-z^2 / 2) / sqrt(2 pi)
+template <typename T> __device__ __forceinline__ float gn_exp_neg(float x) {
+    if constexpr (sizeof(T) == 2) return exp2_hw(x * -1.44269504f);
+    else return expf(-x);
+}
+// with e = exp(-|z|): r = 1 / (1 + e) is s(|z|), e r is s(-|z|), and the derivative of s is their product at either sign
+struct GnSig { float s, slope; };
+template <typename T> __device__ __forceinline__ GnSig gn_sig(float z) {
+    const float e = gn_exp_neg<T>(fabsf(z)), r = gn_rcp<T>(1.f + e);
+    return {z < 0.f ? e * r : r, e * r * r};
+}
+// Phi(z) = erfc(-z / sqrt 2) / 2 and phi(z) = exp(-z^2 / 2) / sqrt(2 pi).  For 16 bits erfc(x) exp(x^2) on x >= 0 is a polynomial in
+// t = 1 / (1 + 0.44 x), fitted over [0, 9.5] to the least largest relative error, 5.2e-6 = 2^-17.5
 template <typename T> __device__ __forceinline__ void gn_phi(float z, float& cdf, float& pdf) {
     if constexpr (sizeof(T) == 4) {
-        cdf = 0.5f * (1.0f + erff(z * 0.70710678118654752f));
+        cdf = 0.5f * erfcf(z * -0.70710678118654752f);
         pdf = 0.3989422804014327f * expf(-0.5f * z * z);
     } else {
         const float x = fabsf(z) * 0.70710678118654752f;
-        const float t = gn_rcp(fmaf(0.3275911f, x, 1.f));
-        const float e = exp2_hw(-x * x * 1.44269504f);
-        const float h = 0.5f * t * e * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
+        const float t = gn_rcp<T>(fmaf(0.44f, x, 1.f));
+        const float e = gn_exp_neg<T>(x * x);
+        float h = fmaf(t, -0.14610421f, 0.35064869f);
+        h = fmaf(t, h, 0.04073489f);
+        h = fmaf(t, h, 0.26358454f);
+        h = fmaf(t, h, 0.24256996f);
+        h = fmaf(t, h, 0.24856098f) * (0.5f * t) * e;
         cdf = z < 0.f ? h : 1.f - h;
         pdf = 0.3989422804014327f * e;
     }
 }
+// tanh(z) = (1 - e) / (1 + e), e = exp(-2 |z|); below 1/8, where 1 - e loses digits, z - z^3 / 3 + 2 z^5 / 15 (the next term is 17 z^6 / 315 of it)
+template <typename T> __device__ __forceinline__ float gn_tanh(float z) {
+    if constexpr (sizeof(T) == 4) return tanhf(z);
+    const float a = fabsf(z), e = gn_exp_neg<T>(2.f * a), q = z * z;
+    const float far = copysignf((1.f - e) * gn_rcp<T>(1.f + e), z), near = z * fmaf(q, fmaf(q, 2.f / 15.f, -1.f / 3.f), 1.f);
+    return a < 0.125f ? near : far;
+}
 template <typename T, int CLS> __device__ __forceinline__ float gn_act(float z, const GnAct& f) {
     if constexpr (CLS == 0) return z > 0.f ? z : f.p0 == 0.f ? (z != z ? z : 0.f) : z * f.p0;
     else if constexpr (CLS == 1) {
-        const float s = gn_sig(f.p0 * z);
-        return fmaf(s, fmaf(f.p1, z, f.p2), f.p3);
-    } else {
+        const float s = gn_sig<T>(z).s;
+        return f.p0 == 0.f ? s : z * s;
+    } else if constexpr (CLS == 2) {
         float cdf, pdf;
         gn_phi<T>(z, cdf, pdf);
         return z * cdf;
-    }
+    } else return gn_tanh<T>(z);
 }
 template <typename T, int CLS> __device__ __forceinline__ float gn_slope(float z, const GnAct& f) {
     if constexpr (CLS == 0) return z > 0.f ? 1.f : z != z ? z : f.p0;
     else if constexpr (CLS == 1) {
-        const float s = gn_sig(f.p0 * z);
-        return fmaf(f.p0 * s * (1.f - s), fmaf(f.p1, z, f.p2), f.p1 * s);
-    } else {
+        const GnSig g = gn_sig<T>(z);
+        return f.p0 == 0.f ? g.slope : fmaf(z, g.slope, g.s);
+    } else if constexpr (CLS == 2) {
         float cdf, pdf;
         gn_phi<T>(z, cdf, pdf);
         return fmaf(z, pdf, cdf);
-    }
+    } else return 4.f * gn_sig<T>(2.f * z).slope;
 }
 
 struct GnArgs {
@@ -735,7 +758,8 @@ template <typename T> void gn_backward_launch(const GnArgs& a, const GnSlab& b, 
     do {                             \
         if (a.act.cls == 0) GO(0);   \
         else if (a.act.cls == 1) GO(1); \
-        else GO(2);                  \
+        else if (a.act.cls == 2) GO(2); \
+        else GO(3);                  \
     } while (0)
 #ifdef GN_INSTANTIATE
 template <typename T> void gn_forward_launch(const GnArgs& a, const GnSlab& b, int threads, int r, bool al, float* stats, float eps,

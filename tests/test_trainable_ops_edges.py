@@ -253,3 +253,38 @@ def test_gpu_softmax_rel_bias_pitched_rows_beyond_32_bits_of_elements(case):
     dx, dt = rs.backward(dyd, xd, stats, td, plan, 0.7)
     _within(dx, ref["dx"], ref["dx_tol"], "dx")
     _within(dt, ref["dtable"], ref["dtable_tol"], "dtable")
+
+
+# ------------------------------------------------------------------------------------------------ activations, relative to their values
+@pytest.mark.parametrize("c", [128, 1024], ids=["one launch", "streamed"])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=lambda t: str(t)[6:])
+@pytest.mark.parametrize("act", ["sigmoid", "silu", "tanh", "gelu"])
+def test_group_norm_activation_relative_to_its_value(dev, act, dtype, c):
+    """weight 0 and the bias as argument: y is act(bias) and dbias its derivative (times dy = 1, in float for every type) and nothing else.
+
+    Bounds in roundings of the value: float tensors exp and division 2 steps each, 1 + e and products 1 each, tanh 4, erfc 16 and its
+    argument's rounding, which erfc carries on z^2 times, twice.  16-bit tensors 2^-16 for all of it, and the output's own half step.  A derivative that
+    crosses zero: relative to its two terms."""
+    kind = getattr(L, "ACT_" + act.upper())
+    g = _gen(c)
+    z = torch.cat([torch.pow(10.0, torch.linspace(-9, 1, c // 4)), -torch.pow(10.0, torch.linspace(-9, 1, c // 4)), torch.linspace(-12.5, 12.5, c // 2)])
+    x = torch.randn(1, 1, c, generator=g).to(dtype).to(dev)
+    w, b = torch.zeros(c, device=dev), z.to(dev)
+    y, stats = gn.forward(x, 1, w, b, kind)
+    dx, dw, db = gn.backward(torch.ones_like(x), x, stats, 1, w, b, kind)
+    zd = z.double()
+    ref, slope = orc.act(zd, kind), orc.act_slope(zd, kind)
+    if act == "tanh":
+        slope = 1 / torch.cosh(zd) ** 2                      # (1 - tanh^2 has no digits left where tanh is 1)
+    if act == "gelu":
+        parts = 0.5 * torch.special.erfc(-zd / math.sqrt(2)) + (zd * torch.exp(-zd * zd / 2)).abs() / math.sqrt(2 * math.pi)
+    elif act == "silu":
+        parts = torch.sigmoid(zd) + (zd * torch.sigmoid(zd) * torch.sigmoid(-zd)).abs()
+    else:
+        parts = slope
+    rel = (24 + 4 * zd * zd) * orc.U if act == "gelu" else torch.full_like(zd, 16 * orc.U)
+    if dtype != F32:
+        rel = torch.full_like(zd, 2.0 ** -16)
+    _within(y.view(-1), ref, ref.abs() * rel + (orc.rounding(ref, dtype) if dtype != F32 else 0) + 2.0 ** -126, "y")
+    _within(db, slope, parts * rel + 2.0 ** -126, "slope")
+    assert float(dx.abs().max()) == 0
