@@ -8,8 +8,9 @@
 //   p = exp(v - max) / sum from the scores again (never from the rounded y),  ds = p * (dy - sum p dy),  dx = scale * ds,
 //   dtable[k][h] = sum of ds over the samples and the pairs whose slot has bucket k
 //
-// exp(d) of a difference d <= 0 is the hardware's 2^(d log2 e): two instructions where a library exponential takes a dozen.  It is off by
-// |d| / 2 steps of float relative to itself -- nothing next to the row's largest value, which has d = 0.
+// exp(d) of a difference d <= 0 is the hardware's 2^(d log2 e): two instructions where a library exponential takes a dozen.  That is off by
+// |d| / 2 steps of float relative to itself, which 16-bit outputs do not see; float outputs (float probabilities, gradients of float scores)
+// take six more instructions that put the lost part back (rs_exp).
 //
 // Bytes bind: every score is read once and every output written once; a row stays in registers in between.  The table is expanded once
 // per call to [head][slot], where the bias of a row is a window whose rows are contiguous.  Four forms, by the row's length M:
@@ -82,8 +83,14 @@ struct RsArgs {
 
 __device__ __forceinline__ int rs_row_of(const RsArgs& a, int j) { return (int)rs_div((unsigned)j, a.by_kw); }
 
-// exp(d), d <= 0 (-inf: 0; a NaN stays one)
-__device__ __forceinline__ float rs_exp(float d) { return exp2_hw(d * 1.44269504f); }
+// exp(d), d <= 0 (-inf: 0; a NaN stays one).  OUT: the type of what is computed from it.  For float the rounding of t = d log2 e and the tail
+// of the constant, |d| / 2 steps of the result together, are put back (two steps are left); an output of 16 bits does not see them.
+template <typename OUT> __device__ __forceinline__ float rs_exp(float d) {
+    const float t = d * 1.44269504f, y = exp2_hw(t);
+    if constexpr (sizeof(OUT) == 2) return y;
+    const float lost = fmaf(d, 1.92596299e-8f, fmaf(d, 1.44269504f, -t)) * 0.69314718f;
+    return fmaf(y, t >= -150.f ? lost : 0.f, y);            // (-inf, and a t that overflowed: lost is a NaN, y is 0)
+}
 
 // position of a row, advanced row by row
 struct RsPos {
@@ -123,14 +130,14 @@ template <int T> __device__ __forceinline__ float rs_max(float v) {
 }
 // joins the waves of a row: (m, s) of a wave -> of the row, and the factor exp(max of the wave - max of the row).  Lane l of every 16
 // takes wave l's pair.  red: two buffers in turn (a wave writes one again only after the barrier of the other)
-template <int WAVES> __device__ __forceinline__ float rs_join(float& m, float& s, const float (*red)[2]) {
+template <typename OUT, int WAVES> __device__ __forceinline__ float rs_join(float& m, float& s, const float (*red)[2]) {
     static_assert(WAVES <= 16, "a pair per lane of a DPP row");
     const int l = threadIdx.x & 15;
     const float ml = l < WAVES ? red[l & (WAVES - 1)][0] : -INFINITY, sl = l < WAVES ? red[l & (WAVES - 1)][1] : 0.f;
     const float top = row_max(ml), z = top == -INFINITY ? 0.f : top;
-    const float f = rs_exp(m - z);
+    const float f = rs_exp<OUT>(m - z);
     m = top;
-    s = row_sum(sl * rs_exp(ml - z));
+    s = row_sum(sl * rs_exp<OUT>(ml - z));
     return f;
 }
 // the same for plain sums
@@ -200,7 +207,7 @@ __global__ __launch_bounds__(T < RS_BLOCK ? RS_BLOCK : T) void rs_forward_kernel
             s[q] = 0.f;
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                v[q][i] = rs_exp(v[q][i] - top);
+                v[q][i] = rs_exp<TY>(v[q][i] - top);
                 s[q] += v[q][i];
             }
             s[q] = rs_sum<T>(s[q]);
@@ -213,7 +220,7 @@ __global__ __launch_bounds__(T < RS_BLOCK ? RS_BLOCK : T) void rs_forward_kernel
 #pragma unroll
         for (int q = 0; q < ROWS; ++q) {
             float f = 1.f;
-            if constexpr (WAVES > 1) f = rs_join<WAVES>(m[q], s[q], red[par][q]);
+            if constexpr (WAVES > 1) f = rs_join<TY, WAVES>(m[q], s[q], red[par][q]);
             if (r + q >= r1) continue;
             const float inv = s[q] == 0.f ? 0.f : 1.f / s[q];
             f *= inv;
@@ -375,7 +382,7 @@ __global__ __launch_bounds__(T < RS_BLOCK ? RS_BLOCK : T) void rs_forward_vec_ke
             for (int i = 0; i < NC; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    v[q][i][e] = rs_exp(v[q][i][e] - top);
+                    v[q][i][e] = rs_exp<TY>(v[q][i][e] - top);
                     s[q] += v[q][i][e];
                 }
             s[q] = wave_sum(s[q]);
@@ -388,7 +395,7 @@ __global__ __launch_bounds__(T < RS_BLOCK ? RS_BLOCK : T) void rs_forward_vec_ke
 #pragma unroll
         for (int q = 0; q < NQ; ++q) {
             float f = 1.f;
-            if constexpr (WAVES > 1) f = rs_join<WAVES>(m[q], s[q], red[par][q]);
+            if constexpr (WAVES > 1) f = rs_join<TY, WAVES>(m[q], s[q], red[par][q]);
             if (q >= nq) continue;
             const float inv = s[q] == 0.f ? 0.f : 1.f / s[q];
             f *= inv;
@@ -444,14 +451,14 @@ template <typename TX, typename TY, int PHASE> __global__ __launch_bounds__(512)
     const float top = m == -INFINITY ? 0.f : m;
     if (PHASE == 1) {
         double all = 0.0;                                    // (a row may have 2^17 tiles)
-        for (int k = 0; k < a.tiles; ++k) all += (double)(part[2 * k + 1] * rs_exp(part[2 * k] - top));
+        for (int k = 0; k < a.tiles; ++k) all += (double)(part[2 * k + 1] * rs_exp<TY>(part[2 * k] - top));
         s = (float)all;
         inv = s == 0.f ? 0.f : 1.f / s;
         TY* y = (TY*)a.y + r * a.ldy;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int j = tile * RS_TILE + t + i * T;
-            if (j < a.M) y[j] = to_elem<TY>(rs_exp(v[i] - top) * inv);
+            if (j < a.M) y[j] = to_elem<TY>(rs_exp<TY>(v[i] - top) * inv);
         }
         if (tile == a.tiles - 1)
             for (int j = a.M + t; j < a.zero_to; j += T) y[j] = to_elem<TY>(0.f);
@@ -462,7 +469,7 @@ template <typename TX, typename TY, int PHASE> __global__ __launch_bounds__(512)
         return;
     }
 #pragma unroll
-    for (int i = 0; i < NV; ++i) s += rs_exp(v[i] - top);
+    for (int i = 0; i < NV; ++i) s += rs_exp<TY>(v[i] - top);
     s = wave_sum(s);
     if ((t & 63) == 0) red[t >> 6] = s;
     __syncthreads();
@@ -551,7 +558,7 @@ __global__ __launch_bounds__(T < 64 ? RS_BLOCK : T) void rs_backward_kernel(RsAr
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 const float v = live && in[i] ? p[q][i] : -INFINITY;
-                p[q][i] = rs_exp(v - top) * inv;
+                p[q][i] = rs_exp<TX>(v - top) * inv;
                 d[q][i] = v == -INFINITY ? 0.f : d[q][i];
                 dot[q] += p[q][i] * d[q][i];
             }
@@ -698,7 +705,7 @@ template <typename TX, typename TY, int T, int NC, int NQ> __global__ __launch_b
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             const float v = p[q][i][e];
-                            p[q][i][e] = rs_exp(v - top[q]) * inv[q];
+                            p[q][i][e] = rs_exp<TX>(v - top[q]) * inv[q];
                             d[q][i][e] = v == -INFINITY ? 0.f : d[q][i][e];
                             dot[q] = fmaf(p[q][i][e], d[q][i][e], dot[q]);
                         }

@@ -288,3 +288,25 @@ def test_group_norm_activation_relative_to_its_value(dev, act, dtype, c):
     _within(y.view(-1), ref, ref.abs() * rel + (orc.rounding(ref, dtype) if dtype != F32 else 0) + 2.0 ** -126, "y")
     _within(db, slope, parts * rel + 2.0 ** -126, "slope")
     assert float(dx.abs().max()) == 0
+
+
+# ------------------------------------------------------------------------------------------------ small probabilities of float scores
+# every form of the kernels: 16 lanes, four columns of four or two queries, column by column, tiles
+@pytest.mark.parametrize("q,k", [((1, 2), (1, 100)), ((1, 5), (1, 400)), ((1, 3), (1, 1500)), ((1, 1), (1, 300)), ((2, 2), (9, 101)), ((1, 2), (1, 17000))],
+                         ids=lambda v: str(v).replace(" ", ""))
+def test_softmax_rel_bias_small_probabilities_keep_their_digits(dev, q, k):
+    """Scores that are exact in float, one 0 and the others down to -85: the exponential of every difference is good to two steps (four
+    roundings) relative to itself, the sum and the inverse add 16, the gradient's two products and difference three."""
+    m = k[0] * k[1]
+    x = -(torch.arange(m) % 680).float() / 8
+    x = x.view(1, 1, 1, m).expand(1, 1, q[0] * q[1], m).contiguous()
+    plan = rs.RelativeBuckets(q, k, torch.zeros(q[0] + k[0] - 1, q[1] + k[1] - 1, dtype=torch.int64, device=dev), 1)
+    table = torch.zeros(1, 1, device=dev)
+    y, stats = rs.forward(x.to(dev), table, plan)
+    p = torch.softmax(x.double(), -1)
+    _within(y, p, p * (20 * orc.U) + 2.0 ** -126, "y")
+    dy = torch.where(torch.arange(m) % 680 == 0, 0.0, 1.0).expand_as(x).contiguous()       # (the gradient of the small ones is no difference)
+    dot = (p * dy).sum(-1, keepdim=True)
+    for t in (F32, BF16):                                   # (probabilities of 16 bits: the scores' gradient is float all the same)
+        dx, _ = rs.backward(dy.to(t).to(dev), x.to(dev), stats, table, plan)
+        _within(dx, p * (dy - dot), p * (24 * orc.U) * (dy - dot).abs() + p * dot * 32 * orc.U + 2.0 ** -126, "dx")
