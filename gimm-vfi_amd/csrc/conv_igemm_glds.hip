@@ -1124,6 +1124,7 @@ extern "C" int gvfi_conv2d_glds_plan(const gvfi_conv_params* pp, int* plan) {
 
 extern "C" int gvfi_conv2d_glds(const gvfi_conv_params* pp, void* stream) {
     const gvfi_conv_params& p = *pp;
+    if (!gvfi_conv_act_ok(p)) return -2;
     int plan[5];
     const int rc = gvfi_conv2d_glds_plan(pp, plan);
     if (rc) return rc;
@@ -1198,7 +1199,7 @@ extern "C" int gvfi_conv2d_pair(const gvfi_conv_params* pa, const gvfi_conv_para
     int plan[5];
     for (int i = 0; i < 2; ++i) {
         const gvfi_conv_params& p = *ps[i];
-        if (p.w_layout != 2 || p.dtype != pa->dtype || p.dtype == GVFI_F32 || p.groups > 1 || p.stats != nullptr) return -2;
+        if (!gvfi_conv_act_ok(p) || p.w_layout != 2 || p.dtype != pa->dtype || p.dtype == GVFI_F32 || p.groups > 1 || p.stats != nullptr) return -2;
         if (((p.algo & 15) != 2 && (p.algo & 15) != 0) || gvfi_conv2d_glds_plan(&p, plan) != 0) return -2;
         if (plan[0] != 6 || plan[1] != 64 || plan[2] != 128) return -2;
         if (((uintptr_t)p.x0 & 15) || ((uintptr_t)p.x1 & 15) || ((uintptr_t)p.w & 15)) return -3;

@@ -293,6 +293,8 @@ __device__ __forceinline__ void act8(float (&v)[8], int act, const float* slope,
 struct GroupConst {
     float bias[8], s1[8], s2[8];
 };
+// the epilogues have every activation but SiLU (GVFI_ACT_SILU is gvfi_group_norm's)
+static inline bool gvfi_conv_act_ok(const gvfi_conv_params& p) { return p.act1 != GVFI_ACT_SILU && p.act2 != GVFI_ACT_SILU; }
 __device__ __forceinline__ void act8s(float (&v)[8], int act, const float (&s)[8]) {
     // one branch per 8 values, never per element
     switch (act) {

@@ -411,7 +411,7 @@ extern "C" int gvfi_conv2d_patch(const gvfi_conv_params* pp, void* stream) {
     const gvfi_conv_params& p = *pp;
     PatchArgs a;
     const int shm = patch_plan(p, a);
-    if (shm == 0) return -2;
+    if (shm == 0 || !gvfi_conv_act_ok(p)) return -2;
     if (((uintptr_t)p.x0 & 15) || ((uintptr_t)p.w & 15)) return -3;
     hipStream_t st = (hipStream_t)stream;
     // persistent workgroups: one per CU and round (every workgroup stages the weights once)

@@ -310,3 +310,24 @@ def test_softmax_rel_bias_small_probabilities_keep_their_digits(dev, q, k):
     for t in (F32, BF16):                                   # (probabilities of 16 bits: the scores' gradient is float all the same)
         dx, _ = rs.backward(dy.to(t).to(dev), x.to(dev), stats, table, plan)
         _within(dx, p * (dy - dot), p * (24 * orc.U) * (dy - dot).abs() + p * dot * 32 * orc.U + 2.0 ** -126, "dx")
+
+
+# ------------------------------------------------------------------------------------------------ SiLU outside group norm
+def test_silu_is_refused_by_every_entry_point_of_the_convolutions(simlib):
+    """A convolution that the LDS-DMA kernel takes, called by its own entry points: their epilogues know no SiLU (and would take its number
+    for another function's)."""
+    import ctypes as C
+
+    from gimmvfi_hip.ops import ConvLayer, Runtime
+
+    rt = Runtime(simlib, "bf16", "cpu")
+    x, w = torch.randn(1, 4, 8, 64, generator=_gen(1)).to(BF16), torch.randn(32, 64, 1, 1, generator=_gen(2)) / 8
+    layer, out = ConvLayer(rt, w, None), torch.zeros(1, 4, 8, 32, dtype=BF16)
+    for kw in (dict(act1=L.ACT_SILU), dict(act2=L.ACT_SILU), {}):
+        p = rt.conv(layer, x, out, algo=2, _defer=True, **kw)[0]
+        entries = [simlib.conv2d, simlib.conv2d_glds] + [simlib.conv2d_patch, simlib.conv2d_col7, simlib.conv2d_p3x3, simlib.conv2d_p3x3s] * bool(kw)
+        for f in entries:
+            assert f(C.byref(p), None) == (-2 if kw else 0)
+        if kw:
+            assert simlib.conv2d_pair(C.byref(p), C.byref(p), None) == -2
+            assert bool((out == 0).all())
