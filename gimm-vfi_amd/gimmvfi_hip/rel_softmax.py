@@ -27,33 +27,35 @@ def _pair(g, name):
 class RelativeBuckets:
     """The buckets of every offset between a query grid and a key grid: ``buckets[dy + qh - 1, dx + qw - 1]`` for dy = jy - iy in
     [-(qh - 1), kh - 1], dx likewise; shape (qh + kh - 1, qw + kw - 1), any integer type, values in [0, num_buckets).  Made once
-    (it looks at the values, and sorts them for the gradient) and kept beside the weights, on the device of ``buckets``."""
+    (it looks at the values, and sorts them for the gradient) and kept beside the weights, on the device of ``buckets``.
+    gradient False: not sorted -- for a program that makes a plan per step (a memory that grows) and never asks for dtable."""
 
-    def __init__(self, q_grid, k_grid, buckets, num_buckets):
+    def __init__(self, q_grid, k_grid, buckets, num_buckets, gradient=True):
         self.qh, self.qw = _pair(q_grid, "q_grid")
         self.kh, self.kw = _pair(k_grid, "k_grid")
         self.num_buckets = int(num_buckets)
         shape = (self.qh + self.kh - 1, self.qw + self.kw - 1)
         if buckets.shape != shape or buckets.is_floating_point() or buckets.dtype == torch.bool:
             raise ValueError(f"buckets must be integers of shape {shape}, got {buckets.dtype} {tuple(buckets.shape)}")
-        if not 1 <= self.num_buckets < 1 << 31 or int(buckets.min()) < 0 or int(buckets.max()) >= self.num_buckets:
-            raise ValueError(f"buckets must lie in [0, {self.num_buckets})")
         flat = buckets.reshape(-1).to(torch.int64)
-        order = torch.sort(flat, stable=True).indices
-        counts = torch.bincount(flat, minlength=self.num_buckets)
-        starts = torch.zeros(self.num_buckets + 1, dtype=torch.int64, device=flat.device)
-        starts[1:] = torch.cumsum(counts, 0)
-        self.bucket_of, self.order, self.starts = (t.to(torch.int32).contiguous() for t in (flat, order, starts))
+        low, high = torch.stack(torch.aminmax(flat)).tolist()            # (the only time that the host waits for the device)
+        if not 1 <= self.num_buckets < 1 << 31 or low < 0 or high >= self.num_buckets:
+            raise ValueError(f"buckets must lie in [0, {self.num_buckets})")
+        self.bucket_of, self.order, self.starts = flat.to(torch.int32).contiguous(), None, None
+        if gradient:
+            by_bucket, order = torch.sort(flat, stable=True)
+            starts = torch.searchsorted(by_bucket, torch.arange(self.num_buckets + 1, device=flat.device))
+            self.order, self.starts = order.to(torch.int32), starts.to(torch.int32)
 
     @classmethod
-    def per_offset(cls, q_grid, k_grid, device=None):
+    def per_offset(cls, q_grid, k_grid, device=None, gradient=True):
         """A bucket of its own for every offset: windows, and attention over a feature map."""
         (qh, qw), (kh, kw) = _pair(q_grid, "q_grid"), _pair(k_grid, "k_grid")
         ny, nx = qh + kh - 1, qw + kw - 1
-        return cls(q_grid, k_grid, torch.arange(ny * nx, device=device).reshape(ny, nx), ny * nx)
+        return cls(q_grid, k_grid, torch.arange(ny * nx, device=device).reshape(ny, nx), ny * nx, gradient)
 
     @classmethod
-    def logarithmic(cls, queries, keys, num_buckets=32, far=128, two_sided=True, first_query=None, device=None):
+    def logarithmic(cls, queries, keys, num_buckets=32, far=128, two_sided=True, first_query=None, device=None, gradient=True):
         """Sequences: near distances have a bucket each, far ones share logarithmic buckets up to distance ``far``, everything
         beyond is in the last.  two_sided: half of the buckets for keys behind the query; else keys behind it share bucket 0.
         first_query: position of the first query among the keys (None: the queries are the last positions)."""
@@ -71,12 +73,12 @@ class RelativeBuckets:
         b = torch.where(d < near, d, (near + steps).clamp(max=half - 1))
         if two_sided:
             b = b + half * (rel > 0)
-        return cls((1, queries), (1, keys), b.reshape(1, -1).to(device), num_buckets)
+        return cls((1, queries), (1, keys), b.reshape(1, -1).to(device), num_buckets, gradient)
 
     def to(self, device):
         new = object.__new__(RelativeBuckets)
         new.__dict__.update(self.__dict__)
-        new.bucket_of, new.order, new.starts = (t.to(device) for t in (self.bucket_of, self.order, self.starts))
+        new.bucket_of, new.order, new.starts = (None if t is None else t.to(device) for t in (self.bucket_of, self.order, self.starts))
         return new
 
 
@@ -134,6 +136,8 @@ def backward(dy, x, stats, table, plan, scale=1.0, key_mask=None, table_grad=Tru
         raise ValueError(f"dy must have x's shape and device, got {tuple(dy.shape)} on {dy.device}")
     if stats.dtype != torch.float32 or stats.shape != (b, h, q, 2) or not stats.is_contiguous() or stats.get_device() != x.get_device():
         raise ValueError("stats must be what forward() returned for x")
+    if table_grad and plan.order is None:
+        raise ValueError("the plan was made with gradient=False")
     ldx, ldd = rows.pitch_of(x, "x"), rows.pitch_of(dy, "dy")
     dx = rows.new_like(x)
     dtable = torch.empty_like(table) if table_grad else None
@@ -141,7 +145,7 @@ def backward(dy, x, stats, table, plan, scale=1.0, key_mask=None, table_grad=Tru
         return dx, None if dtable is None else dtable.zero_()
     ws = rows.workspace(x, lib.softmax_rel_bias_workspace, "softmax_rel_bias", b, h, plan.qh, plan.qw, plan.kh, plan.kw, 1)
     rows.launch(lib.softmax_rel_bias_backward, x, "softmax_rel_bias_backward", dy.data_ptr(), ldd, x.data_ptr(), xt, ldx, table.data_ptr(), plan.bucket_of.data_ptr(),
-                plan.num_buckets, plan.order.data_ptr(), plan.starts.data_ptr(),
+                plan.num_buckets, plan.order.data_ptr() if table_grad else None, plan.starts.data_ptr() if table_grad else None,
                 None if key_mask is None else key_mask.data_ptr(), float(scale), stats.data_ptr(),
                 dx.data_ptr(), m, None if dtable is None else dtable.data_ptr(), b, h, plan.qh,
                 plan.qw, plan.kh, plan.kw, ws.data_ptr(), dt)
@@ -167,4 +171,6 @@ class _SoftmaxRelBias(torch.autograd.Function):
 def softmax_rel_bias(x, table, plan, scale=1.0, key_mask=None, dtype=None):
     """y of forward(), recorded for autograd."""
     rows.refuse_captured_leaves("softmax_rel_bias", x, table)
+    if plan.order is None and table.requires_grad and torch.is_grad_enabled():
+        raise ValueError("table requires a gradient, and the plan was made with gradient=False")
     return _SoftmaxRelBias.apply(x, table, plan, scale, key_mask, dtype)

@@ -331,3 +331,22 @@ def test_silu_is_refused_by_every_entry_point_of_the_convolutions(simlib):
         if kw:
             assert simlib.conv2d_pair(C.byref(p), C.byref(p), None) == -2
             assert bool((out == 0).all())
+
+
+# ------------------------------------------------------------------------------------------------ plans
+def test_plan_without_the_gradients_tables(dev):
+    """A program that never asks for the table's gradient gets its plan without a sort; asked for all the same, it is refused."""
+    for make in (lambda **kw: rs.RelativeBuckets.logarithmic(2, 70, device=dev, **kw), lambda **kw: rs.RelativeBuckets.per_offset((1, 2), (1, 70), device=dev, **kw),
+                 lambda **kw: rs.RelativeBuckets((1, 2), (1, 70), torch.arange(71, device=dev).view(1, 71) % 9, 9, **kw)):
+        full, plan = make(), make(gradient=False).to(dev)
+        assert plan.order is None and plan.starts is None and torch.equal(plan.bucket_of, full.bucket_of)
+        assert full.starts.tolist() == [int((full.bucket_of < k).sum()) for k in range(full.num_buckets + 1)]
+        table, x = torch.randn(plan.num_buckets, 2, generator=_gen(1)).to(dev), torch.randn(1, 2, 2, 70, generator=_gen(2)).to(dev)
+        y, stats = rs.forward(x, table, plan)
+        assert torch.equal(y, rs.forward(x, table, full)[0])
+        assert torch.equal(rs.backward(y, x, stats, table, plan, table_grad=False)[0], rs.backward(y, x, stats, table, full)[0])
+        with pytest.raises(ValueError, match="gradient=False"):
+            rs.backward(y, x, stats, table, plan)
+        with pytest.raises(ValueError, match="gradient=False"):
+            rs.softmax_rel_bias(x, table.clone().requires_grad_(), plan)
+        assert torch.equal(rs.softmax_rel_bias(x, table, plan), y)
