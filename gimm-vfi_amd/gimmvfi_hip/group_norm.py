@@ -19,6 +19,16 @@ from . import rows
 
 ACTS = (L.ACT_NONE, L.ACT_RELU, L.ACT_LRELU, L.ACT_SIGMOID, L.ACT_TANH, L.ACT_GELU, L.ACT_SILU)
 
+LAUNCH = 1 << 23        # (image, group) pairs below which one launch stays, seven images rounded up; larger batches go out in several
+
+
+def _batches(n, c, groups):
+    """(first image, images) of every call: as many as the library takes in one."""
+    step = min((LAUNCH - 1) // groups - 7, LAUNCH - 1, 128 * ((1 << 24) // ((c + 15) // 16) - 1))
+    if n <= step or step < 1:
+        return ((0, n),)
+    return [(lo, min(step, n - lo)) for lo in range(0, n, step)]
+
 
 def _sizes(x, groups, act, name):
     if x.dim() < 2:
@@ -45,9 +55,11 @@ def forward(x, groups, weight=None, bias=None, act=L.ACT_NONE, eps=1e-5, out=Non
     stats = x.new_empty((n, groups, 2), dtype=torch.float32)
     if x.numel() == 0:
         return out, stats.zero_()
-    ws = rows.workspace(x, lib.group_norm_workspace, "group_norm", c, groups, n, hw)
-    rows.launch(lib.group_norm, x, "group_norm", x.data_ptr(), ldx, c, groups, n, hw, w, b, float(eps), act, out.data_ptr(), ldy, stats.data_ptr(),
-                ws.data_ptr(), dt)
+    es = x.element_size()
+    for lo, k in _batches(n, c, groups):
+        ws = rows.workspace(x, lib.group_norm_workspace, "group_norm", c, groups, k, hw)
+        rows.launch(lib.group_norm, x, "group_norm", x.data_ptr() + lo * hw * ldx * es, ldx, c, groups, k, hw, w, b, float(eps), act,
+                    out.data_ptr() + lo * hw * ldy * es, ldy, stats.data_ptr() + lo * groups * 8, ws.data_ptr(), dt)
     return out, stats
 
 
@@ -67,10 +79,16 @@ def backward(dy, x, stats, groups, weight=None, bias=None, act=L.ACT_NONE, param
     db = x.new_empty(c, dtype=torch.float32) if param_grads else None
     if x.numel() == 0:
         return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_()
-    ws = rows.workspace(x, lib.group_norm_workspace, "group_norm", c, groups, n, hw)
-    rows.launch(lib.group_norm_backward, x, "group_norm_backward", dy.data_ptr(), ldd, x.data_ptr(), ldx, c, groups, n, hw, w, b, stats.data_ptr(), act,
-                dx.data_ptr(), c, None if dw is None else dw.data_ptr(),
-                None if db is None else db.data_ptr(), ws.data_ptr(), dt)
+    es = x.element_size()
+    for lo, k in _batches(n, c, groups):
+        ws = rows.workspace(x, lib.group_norm_workspace, "group_norm", c, groups, k, hw)
+        gw, gb = (dw, db) if lo == 0 or not param_grads else (torch.empty_like(dw), torch.empty_like(db))
+        rows.launch(lib.group_norm_backward, x, "group_norm_backward", dy.data_ptr() + lo * hw * ldd * es, ldd, x.data_ptr() + lo * hw * ldx * es, ldx, c,
+                    groups, k, hw, w, b, stats.data_ptr() + lo * groups * 8, act, dx.data_ptr() + lo * hw * c * es, c,
+                    None if gw is None else gw.data_ptr(), None if gb is None else gb.data_ptr(), ws.data_ptr(), dt)
+        if lo and param_grads:
+            dw.add_(gw)
+            db.add_(gb)
     return dx, dw, db
 
 

@@ -441,7 +441,7 @@ int gvfi_flow_to_image(const float* flow, long long img_stride, int n_img, int h
  * arguments are refused and nothing was launched. */
 /* Group norm with an activation (csrc/group_norm.hip): x [N][HW][ldx], G groups of C / G channels, biased variance;
  * y = act((x - mean) * rstd * gamma + beta), gamma / beta [C] float or NULL (1 / 0), act: none, ReLU, LeakyReLU(0.1), sigmoid, tanh,
- * GELU or SiLU.  stats [N][G][2] float receives mean and rstd = 1 / sqrt(var + eps) for the backward pass.
+ * GELU or SiLU.  (N + 7) * G < 2^23 (a launch has fewer than 2^32 lanes).  stats [N][G][2] float receives mean and rstd = 1 / sqrt(var + eps) for the backward pass.
  * The norm "group" of RAFT's encoders (raft/extractor.py:6-58,122-220), beside gvfi_instnorm_apply. */
 long long gvfi_group_norm_workspace(int C, int G, long long N, long long HW);
 int gvfi_group_norm(const void* x, long long ldx, int C, int G, long long N, long long HW, const float* gamma,

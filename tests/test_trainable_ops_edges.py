@@ -350,3 +350,22 @@ def test_plan_without_the_gradients_tables(dev):
         with pytest.raises(ValueError, match="gradient=False"):
             rs.softmax_rel_bias(x, table.clone().requires_grad_(), plan)
         assert torch.equal(rs.softmax_rel_bias(x, table, plan), y)
+
+
+# ------------------------------------------------------------------------------------------------ more images than one launch takes
+def _many_images(dev, shape, groups, dtype, monkeypatch=None, limit=None):
+    if limit:
+        monkeypatch.setattr(gn, "LAUNCH", limit)
+    _gn_case(dev, shape, groups, L.ACT_SILU, dtype, shape[-1] + 3, 1, True)
+
+
+@pytest.mark.parametrize("shape,groups,limit", [((23, 40), 5, 64), ((9, 3, 2, 16), 2, 32), ((130, 5, 24), 3, 401)], ids=lambda v: str(v).replace(" ", ""))
+def test_group_norm_in_several_calls(dev, monkeypatch, shape, groups, limit):
+    """A batch whose (image, group) pairs are more than a launch takes goes out in several; here with a small limit."""
+    _many_images(dev, shape, groups, F32, monkeypatch, limit)
+
+
+@pytest.mark.gpu
+def test_gpu_group_norm_of_many_rows():
+    """Tokens as images of one pixel, 32 groups: 300000 x 32 pairs pass the 2^23 workgroups of a launch."""
+    _many_images(torch.device("cuda", 0), (300000, 64), 32, BF16)
