@@ -154,10 +154,11 @@ static bool gn_plan(GnArgs& a) {
     const long long n = a.N;
     return n * a.chunks < (1LL << 23) && (n + 7) * a.G < (1LL << 23) && (a.C + 15) / 16 * ((n + GN_IMAGES - 1) / GN_IMAGES) < (1LL << 24);
 }
-// Groups of a workgroup of the one-launch form, and the octets of a lane (0: the image does not fit).  As few groups as give whole
+// Groups of a workgroup of the one-launch form, and the octets of a lane (0: the image does not fit, or streaming is faster; bytes: what the
+// pass reads).  As few groups as give whole
 // octets while the workgroups are few (every workgroup's share is latency then); more, for longer runs of bytes, while there are
 // more than 1024 of them.
-static int gn_slab_plan(const GnArgs& a, int most, GnSlab& b, int& threads) {
+static int gn_slab_plan(const GnArgs& a, int most, double bytes, GnSlab& b, int& threads) {
     int g = 1;
     while (g < a.G && (g * a.Cg) % 8) ++g;
     if ((g * a.Cg) % 8) return 0;
@@ -171,12 +172,18 @@ static int gn_slab_plan(const GnArgs& a, int most, GnSlab& b, int& threads) {
     b.images8 = a.N >= 8 ? (a.N + 7) / 8 : 0;
     threads = a.HW * b.octp <= 1024 ? 256 : 512;
     const long long r = (a.HW * b.octp + threads - 1) / threads;
-    // Up to 4 octets of a lane (a workgroup's time is then below that of the second and third launch) always; more only with enough
-    // workgroups to occupy half of the CUs, where not reading twice pays although a workgroup reads 16 bytes of every pixel:
-    // 16 x 7168 pixels x 96 bfloat16 channels 28 us against 36, 2 x 7168 pixels 26 against 15; beyond 16, 46 against 35
-    // (16 x 14336 pixels x 64 channels).
-    const long long few = 4, many = (long long)a.N * b.runs >= 128 ? 16 : few;
-    return r <= most && r <= many ? (int)r : 0;
+    // Up to 4 octets of a lane (a workgroup's time is then below that of the other launches of the streaming form) always: 16 x 448 pixels x 128
+    // bfloat16 channels 12.6 us against 18.3, 8 x 2048 x 256 12.8 against 23.3 (forward with the call; backward likewise).  More only where not
+    // reading twice pays although a workgroup takes 16 bytes of every pixel and its neighbours the rest of the same lines:
+    //   workgroups for half of the CUs    8 images x 7168 x 32 channels, 32 workgroups, backward 26.3 against 19.8; from 128 on 33.8 against 43.1
+    //   a whole image on one XCD          (8 images, dealt) else every XCD fetches the lines: 6 x 7168 x 512 channels 91.8 against 40.5, 4 x 7168 x
+    //                                     512 57.3 against 35.1; 8 x 7168 x 512 42.6 against 45.3
+    //   XCDs with the same load           9 images x 7168 x 512 72.4 against 50.0 (seven XCDs wait for the one with two)
+    //   128 MB read at most               what the last-level cache holds between one run's visit to a line and the next: 32 x 7168 x 128 (58 MB)
+    //                                     forward 39.9 against 45.2, backward (117 MB) 71.9 against 78.0; 64 x 7168 x 128 backward (235 MB) 174
+    //                                     against 130
+    if (r > 4 && ((long long)a.N * b.runs < 128 || a.N < 8 || 4LL * a.N < 3 * 8 * b.images8 || bytes > 128e6)) return 0;
+    return r <= most ? (int)r : 0;
 }
 extern "C" long long gvfi_group_norm_workspace(int C, int G, long long N, long long HW) {
     if (gn_check(C, G, N, HW, 0, GVFI_F32) || N >= (1LL << 30)) return -2;
@@ -199,7 +206,7 @@ extern "C" int gvfi_group_norm(const void* x, long long ldx, int C, int G, long 
     const bool al = C % 8 == 0 && gvfi_rows_aligned(x, ldx, es) && gvfi_rows_aligned(y, ldy, es);
     GnSlab b = {};
     int threads = 0;
-    const int r = al ? gn_slab_plan(a, dtype == GVFI_F32 ? 8 : 16, b, threads) : 0;
+    const int r = al ? gn_slab_plan(a, dtype == GVFI_F32 ? 8 : 16, (double)N * HW * C * es, b, threads) : 0;
     GVFI_DISPATCH_T(dtype, gn_forward_launch<T>(a, b, threads, r, al, stats, eps, (hipStream_t)stream));
     return (int)hipGetLastError();
 }
@@ -220,7 +227,7 @@ extern "C" int gvfi_group_norm_backward(const void* dy, long long lddy, const vo
     const bool al = C % 8 == 0 && gvfi_rows_aligned(x, ldx, es) && gvfi_rows_aligned(dy, lddy, es) && gvfi_rows_aligned(dx, lddx, es);
     GnSlab b = {};
     int threads = 0;
-    const int r = al ? gn_slab_plan(a, dtype == GVFI_F32 ? 8 : 16, b, threads) : 0;
+    const int r = al ? gn_slab_plan(a, dtype == GVFI_F32 ? 8 : 16, (double)N * HW * C * es * 2, b, threads) : 0;
     hipStream_t st = (hipStream_t)stream;
     GVFI_DISPATCH_T(dtype, gn_backward_launch<T>(a, b, threads, r, al, st));
     if ((dgamma || dbeta) && (r || N > GN_IMAGES)) gn_params(a, st);       // (else the last launch above has done it)
