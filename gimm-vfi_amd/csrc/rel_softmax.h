@@ -800,15 +800,16 @@ template <typename TX, typename TY> void rs_backward_launch(const RsArgs& a, hip
         else if (a.M <= 4096) GO(512, 2, 4); \
         else GO(512, 4, 2);                  \
     } while (0)
-// The backward pass keeps twice as much per lane, so it takes more lanes (448 columns: 128 lanes 48 us, 64 lanes 58; 1792 columns: 512
-// lanes x 2 queries 191 us, 256 lanes x 4 203).
+// The backward pass keeps twice as much per lane, so it takes more lanes, and above 256 columns two queries at a time.  40 M float scores with
+// bfloat16 gradients, four queries | two, us: 200 columns 108 | 116; 401 114 | 105; 1000 106 | 110; 1500 113 | 110; 2400 123 | 121; 3500 117 | 114;
+// 8160 288 | 181.  bfloat16 scores: 200 86 | 89; 401 80 | 78; 1000 69 | 71; 1500 81 | 81; 2400 92 | 83; 3500 80 | 74; 8160 234 | 134.
 #define RS_VEC_BACKWARD(GO)                  \
     do {                                     \
         if (a.M <= 256) GO(64, 1, 4);        \
-        else if (a.M <= 512) GO(128, 1, 4);  \
-        else if (a.M <= 1024) GO(256, 1, 4); \
+        else if (a.M <= 512) GO(128, 1, 2);  \
+        else if (a.M <= 1024) GO(256, 1, 2); \
         else if (a.M <= 2048) GO(512, 1, 2); \
-        else if (a.M <= 4096) GO(512, 2, 4); \
+        else if (a.M <= 4096) GO(512, 2, 2); \
         else GO(512, 4, 2);                  \
     } while (0)
 
