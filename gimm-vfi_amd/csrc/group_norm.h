@@ -13,9 +13,10 @@
 // pixels and has at most GN_FOLD * GN_MOST of them, the sums over chunks are in double.
 //
 // Measured on one MI355X, whose copy of 1 GiB reaches 5.2 TB/s.  Streaming form, 16 images of 128 x 224 x 64 bfloat16 with ReLU: sums
-// 15.0 us (3.9 TB/s), joining 4.0, applying 24.4 (4.8 TB/s, part of its reads from the caches).  One-launch form, 16 images of
-// 64 x 112 x 96 bfloat16 with SiLU: forward 24.8 us, backward 36.1 (44 and 66 MB: lines per CU bind, every lane takes 16 bytes of
-// a 192-byte pixel); 2 images of 16 x 28 x 128: 6.0.
+// 15.1 us (3.9 TB/s), joining 3.9, applying 24.6 (4.8 TB/s, part of its reads from the caches); a training step 121 us, of 2 images of
+// 1088 x 1920 x 64 907 us (eight passes over 535 MB: 4.7 TB/s).  One-launch form, 16 images of 64 x 112 x 96 bfloat16 with SiLU: forward 26 us, backward 36
+// (44 and 66 MB): every lane takes 16 bytes of a 192-byte pixel, so a line of 128 bytes is asked of the L2 eight times (1.38 M and 2.75 M
+// requests), and the L1 waits for them 0.6 and 0.55 of the time; vector instructions fill 0.4 and 0.5.  2 images of 16 x 28 x 128: 6.2.
 #pragma once
 #include "row_ops.h"
 

@@ -29,9 +29,10 @@
 // by bucket in a fixed order, in double: a bucket may collect millions of terms.
 //
 // Measured on one MI355X (copy of 1 GiB: 5.2 TB/s), float scores, bfloat16 probabilities: 28672 rows of 1792 (32 x 56 map) 59 us =
-// 5.2 TB/s; 8160 rows of 8160 (68 x 120) forward 92 us = 4.3 TB/s, backward 143 us = 4.7 TB/s with the adds into the slabs, 23 + 5 us
-// for the sums over slabs and buckets.  117600 rows of 49 (7 x 7 windows, half): forward 13.4 us, backward 20.6 (1.7 TB/s: instructions
-// bind, a row has 49 columns for 64 places).  Key rows that fours would cross (67 x 121): 125 us forward, column by column.
+// 5.2 TB/s; 8160 rows of 8160 (68 x 120) forward 91 us = 4.4 TB/s, backward 146 us = 4.6 TB/s with the adds into the slabs, 23 + 5 us
+// for the sums over slabs and buckets; the whole step with float probabilities 326 us for 1.33 GB in two passes.  117600 rows of 49 (7 x 7 windows, half):
+// forward 13.6 us, backward 20.6 (1.7 TB/s: instructions bind, a row has 49 columns for 64 places).  Key rows that fours would cross
+// (67 x 121): 125 us forward, column by column, the step 367 us.  Rows in tiles, 544 of 40000 keys: the step 223 us, x and dy read twice.
 #pragma once
 #include "row_ops.h"
 

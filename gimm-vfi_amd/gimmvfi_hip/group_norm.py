@@ -5,7 +5,8 @@ dbias)`` are the two passes; ``group_norm_act(...)`` records them for autograd. 
 any row pitch (a channel slice of a wider buffer; an NCHW tensor in channels_last memory as ``x.permute(0, 2, 3, 1)``); the
 statistics of a group are taken over the middle dimensions and the group's C / groups channels.  weight, bias: (C,) float32 or
 None.  act: ACT_NONE, ACT_RELU, ACT_LRELU (0.1), ACT_SIGMOID, ACT_TANH, ACT_GELU (erf) or ACT_SILU of ``gimmvfi_hip.lib``.
-Outputs are contiguous, in x's type; stats is (N, groups, 2) float32: mean and 1 / sqrt(var + eps).
+Outputs are contiguous, in x's type; stats is (N, groups, 2) float32: mean and 1 / sqrt(var + eps).  Values and derivatives of the
+activations are accurate relative to themselves, to a few steps of float for float32 and to 2**-16 before the rounding for 16 bits.
 
 Both passes can be captured into a graph.  The autograd form refuses leaves that require gradients during a capture (rows.py says
 why).
